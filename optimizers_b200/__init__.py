@@ -67,6 +67,7 @@ from optimizers_b200.config import (
     SVDOrthogonalizationConfig,
     WeightDecayType,
 )
+from optimizers_b200.grad_clip import clip_grad_norm_, grad_norm
 from optimizers_b200.shampoo import DistributedShampoo
 
 

@@ -56,6 +56,9 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--native-backend", choices=["auto", "native", "torch"], default="auto")
     ap.add_argument("--seed", type=int, default=2022)
     ap.add_argument("--window-size", type=int, default=10)
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="scale the gradients to at most this norm before every step")
+    ap.add_argument("--fp8", action="store_true", help="llama: 8-bit operands in the linear layers of every block")
+    ap.add_argument("--fused-embedding", action="store_true", help="gpt2, llama: token embedding and its gradient from this package's kernels")
     ap.add_argument("--checkpoint-dir", default=None)
     ap.add_argument("--metrics-dir", default=None)
     ap.add_argument("--config", default=None, metavar="YAML",
@@ -78,6 +81,14 @@ def parse_args(argv=None) -> argparse.Namespace:
             raise SystemExit(f"unknown keys in {path}: {sorted(unknown)}")
         ap.set_defaults(**preset)
         args = ap.parse_args(argv)
+    if args.max_grad_norm is not None and not args.max_grad_norm >= 0:
+        ap.error(f"--max-grad-norm is at least 0, got {args.max_grad_norm}")
+    if args.max_grad_norm is not None and args.parallelism == "ddp_fused":
+        ap.error("--max-grad-norm needs reduced gradients; ddp_fused reduces them inside the optimizer's step")
+    if args.fp8 and args.model != "llama":
+        ap.error("--fp8 needs --model llama")
+    if args.fused_embedding and args.model not in ("gpt2", "llama"):
+        ap.error("--fused-embedding needs --model gpt2 or llama")
     return args
 
 
@@ -99,8 +110,10 @@ def build_model(args: argparse.Namespace) -> tuple[torch.nn.Module, str]:
         return M.ResNet18(), "image"
     if args.model == "gpt2":
         cfg = M.GPT2Config(vocab_size=1024, n_ctx=args.seq_len, n_layer=2, n_head=4, d_model=128, d_mlp=512) if args.small else M.GPT2Config()
+        cfg.fused_embedding = args.fused_embedding
         return M.GPT2(cfg), "tokens"
     cfg = M.LlamaConfig(vocab_size=1024, n_layer=2, n_head=4, d_model=128, d_ffn=256) if args.small else M.LlamaConfig()
+    cfg.fused_embedding, cfg.fp8 = args.fused_embedding, args.fp8
     return M.Llama(cfg), "tokens"
 
 
@@ -188,6 +201,13 @@ def build_optimizer(args: argparse.Namespace, model: torch.nn.Module, distribute
     return ob.DistributedShampoo(params, **common)
 
 
+def shard_group(args: argparse.Namespace, mesh):
+    """The process group that one gradient is spread over, if any."""
+    if args.parallelism in ("fsdp", "fully_shard"):
+        return dist.group.WORLD
+    return mesh["shard"].get_group() if args.parallelism in ("hsdp", "hybrid_shard") else None
+
+
 def save_checkpoint(path: str, model: torch.nn.Module, optimizer: torch.optim.Optimizer) -> None:
     import torch.distributed.checkpoint as dcp
     from torch.distributed.checkpoint.state_dict import get_state_dict
@@ -255,6 +275,8 @@ def main(argv=None) -> float:
         optimizer.zero_grad(set_to_none=not keep_grads)
         loss = model(x, y) if kind == "tokens" else torch.nn.functional.cross_entropy(model(x), y)
         loss.backward()
+        if args.max_grad_norm is not None:
+            ob.clip_grad_norm_(model.parameters(), args.max_grad_norm, shard_group=shard_group(args, mesh))
         optimizer.step()
         metrics.update(loss)
         metrics.log()

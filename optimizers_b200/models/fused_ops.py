@@ -21,6 +21,14 @@ around library GEMMs.
     fp32 statistics, output directly in the autocast dtype (what the following linear layer
     consumes), backward with a two-stage dgamma / dbeta reduction.
 
+``add_rms_norm``
+    the residual addition and the RMSNorm behind it in one pass: ``h = x + residual`` and the norm of h; the backward pass
+    adds the gradient that reaches h directly (``ops/csrc/residual_norm.cu``; any width up to 16384).
+
+``embedding``
+    table lookup with a scale; the dense gradient of the table is summed over the tokens sorted by their number, in a fixed
+    order and without atomics (``ops/csrc/embed_kernels.cu``).
+
 No reference counterpart (the reference's examples use stock torch modules).
 """
 
@@ -29,6 +37,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 _ENABLED = True
 _EXT = None
@@ -184,6 +193,123 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     xf = x.float()
     y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     return (y * weight.float()).to(x.dtype)
+
+
+# --------------------------------------------------------------------------------------------------
+# Residual addition + RMSNorm
+# --------------------------------------------------------------------------------------------------
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, residual: Tensor, weight: Tensor, eps: float, out_dtype: torch.dtype):  # type: ignore[override]
+        w = weight.contiguous()
+        y, _, h, rstd = _ext().add_norm_fwd(x, residual, w, eps, 1 if out_dtype == torch.bfloat16 else 0, True)
+        _count()
+        ctx.save_for_backward(h, w, rstd)
+        ctx.x_dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor | None, dh: Tensor | None):  # type: ignore[override]
+        h, w, rstd = ctx.saved_tensors
+        if dy is None:  # only the sum was used
+            return (None if dh is None else dh.to(ctx.x_dtype)), dh, (torch.zeros_like(w) if dh is not None else None), None, None
+        if dy.dtype not in (torch.float32, torch.bfloat16):
+            dy = dy.float()
+        dx, dr, dw = _ext().add_norm_bwd(
+            dy.contiguous(), None if dh is None else dh.contiguous(), h, w, rstd, ctx.x_dtype == torch.bfloat16, True
+        )
+        _count()
+        return dx, dr, dw, None, None
+
+
+def _check_add_norm(x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
+    if x.dim() < 1 or weight.shape != x.shape[-1:]:
+        raise ValueError(f"a norm weight of shape {tuple(weight.shape)} does not fit rows of shape {tuple(x.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"x and residual differ in shape: {tuple(x.shape)} and {tuple(residual.shape)}")
+    if any(t is not None and not t.is_floating_point() for t in (x, residual, weight)):
+        raise ValueError("add_rms_norm takes floating-point tensors")
+
+
+def _norm_operands(x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tensor | None]:
+    """Contiguous rows; an fp32 x is added to a residual in fp32."""
+    x2 = x.reshape(-1, x.shape[-1]).contiguous()
+    if residual is None:
+        return x2, None
+    if x.dtype == torch.float32 and residual.dtype == torch.bfloat16:
+        residual = residual.float()
+    return x2, residual.reshape(x2.shape).contiguous()
+
+
+def _add_norm_native(x2: Tensor, r2: Tensor | None, weight: Tensor) -> bool:
+    kinds = (torch.float32, torch.bfloat16)
+    return (
+        _native(x2) and x2.numel() > 0 and x2.dtype in kinds and weight.dtype in kinds and weight.device == x2.device
+        and (r2 is None or (r2.dtype in kinds and r2.device == x2.device)) and x2.shape[1] <= _ext().add_norm_max_width()
+    )
+
+
+def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """``h = x + residual`` in the wider of their types, and ``rms_norm(h, weight)`` over the last dim in the autocast dtype (or
+    x's): ``(y, h)``.  The statistics are those of h as it is returned."""
+    if residual is None:
+        raise ValueError("add_rms_norm needs a residual; rms_norm normalises x alone")
+    _check_add_norm(x, residual, weight)
+    out_dtype = _norm_out_dtype(x)
+    x2, r2 = _norm_operands(x, residual)
+    if _add_norm_native(x2, r2, weight):
+        y, h = _AddNorm.apply(x2, r2, weight, eps, out_dtype)
+        return y.view(x.shape), h.view(x.shape)
+    h = (x.float() + residual.float()).to(torch.promote_types(x.dtype, residual.dtype))
+    hf = h.float()
+    y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps)
+    return (y * weight.float()).to(out_dtype), h
+
+
+# --------------------------------------------------------------------------------------------------
+# Token embedding
+# --------------------------------------------------------------------------------------------------
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids: Tensor, weight: Tensor, scale: float, out_dtype: torch.dtype):  # type: ignore[override]
+        ctx.save_for_backward(ids)
+        ctx.meta = (weight.shape[0], scale, weight.dtype)
+        y = _ext().embed_fwd(ids, weight.contiguous(), scale, out_dtype == torch.bfloat16)
+        _count()
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor):  # type: ignore[override]
+        (ids,) = ctx.saved_tensors
+        rows, scale, dtype = ctx.meta
+        dy = dy.contiguous() if dy.dtype in (torch.float32, torch.bfloat16) else dy.float().contiguous()
+        dw = _ext().embed_bwd(ids, dy, rows, scale, dtype == torch.bfloat16)
+        _count()
+        return None, dw, None, None
+
+
+def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> Tensor:
+    """``scale * weight[ids]`` in ``out_dtype`` (the table's by default), for integer ``ids`` of any shape and a table [V, C].
+
+    The gradient of the table is dense and summed in 32 bits, in the order of the tokens: the same inputs give the same bits.  On
+    the GPU, where a check would make the host wait, a token outside the table gives a row of NaN and takes no part in the
+    gradient; PyTorch on the CPU raises ``IndexError``.
+    """
+    if weight.dim() != 2:
+        raise ValueError(f"an embedding table is a matrix, got shape {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"token numbers are int64 or int32, got {ids.dtype}")
+    out_dtype = weight.dtype if out_dtype is None else out_dtype
+    if not (weight.is_floating_point() and out_dtype.is_floating_point):
+        raise ValueError("embedding takes and returns floating-point tensors")
+    kinds = (torch.float32, torch.bfloat16)
+    if _native(weight) and ids.device == weight.device and weight.dtype in kinds and out_dtype in kinds and weight.numel() > 0:
+        return _Embedding.apply(ids.reshape(-1).contiguous(), weight, float(scale), out_dtype).view(*ids.shape, weight.shape[1])
+    y = F.embedding(ids, weight)
+    return y.to(out_dtype) if scale == 1.0 else (y.float() * scale).to(out_dtype)
 
 
 # --------------------------------------------------------------------------------------------------

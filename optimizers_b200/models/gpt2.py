@@ -4,7 +4,7 @@ d_model 768, 12 heads, MLP 3072, vocabulary 50257, context 1024.
 
 With ``fused=True`` (default) the normalisations and the LM head + cross-entropy go through
 ``optimizers_b200.models.fused_ops`` (CUDA kernels on a GPU, the same formulas in PyTorch
-elsewhere); ``fused=False`` is the stock-module formulation."""
+elsewhere); ``fused=False`` is the stock-module formulation.  ``fused_embedding`` takes the token embedding from there too."""
 
 from __future__ import annotations
 
@@ -27,6 +27,7 @@ class GPT2Config:
     d_model: int = 768
     d_mlp: int = 3072
     fused: bool = True
+    fused_embedding: bool = False
 
 
 class _Block(nn.Module):
@@ -82,7 +83,8 @@ class GPT2(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         B, T = idx.shape
         pos = torch.arange(T, device=idx.device)
-        x = self.wte(idx) + self.wpe(pos)
+        tokens = fused_ops.embedding(idx, self.wte.weight) if self.cfg.fused_embedding else self.wte(idx)
+        x = tokens + self.wpe(pos)
         for blk in self.blocks:
             x = blk(x)
         if self.cfg.fused:

@@ -3,7 +3,10 @@ head.  Defaults are the 1B configuration of the benchmarks: 16 layers, d_model 2
 FFN 8192, vocabulary 32000.
 
 With ``fused=True`` (default) RMSNorm and the head + cross-entropy go through
-``optimizers_b200.models.fused_ops``."""
+``optimizers_b200.models.fused_ops``.  ``fused_embedding`` takes the token embedding from there too.
+``fp8`` runs the seven linear layers of a block on 8-bit operands (``optimizers_b200.models.fp8``) and joins every residual
+addition with the RMSNorm behind it; without gradients the norms hand their rows over in 8 bits, and
+``hold_fp8_weights()`` keeps the weights in 8 bits between calls."""
 
 from __future__ import annotations
 
@@ -13,7 +16,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from optimizers_b200.models import fused_ops
+from optimizers_b200.models import fp8, fused_ops
 
 
 @dataclass
@@ -27,6 +30,8 @@ class LlamaConfig:
     rope_theta: float = 10000.0
     norm_eps: float = 1e-5
     fused: bool = True
+    fused_embedding: bool = False
+    fp8: bool = False
 
 
 class RMSNorm(nn.Module):
@@ -81,6 +86,35 @@ class _Layer(nn.Module):
         h = self.ffn_norm(x)
         return x + self.w_down(F.silu(self.w_gate(h)) * self.w_up(h))
 
+    _LINEARS = ("wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down")
+
+    def _fp8(self, x, out_dtype: torch.dtype, *names: str):
+        held = None if torch.is_grad_enabled() else getattr(self, "_held", None)
+        return fp8.linear(x, tuple(getattr(self, n).weight if held is None else held[n] for n in names), out_dtype)
+
+    def forward_fp8(self, branch: torch.Tensor | None, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
+        """The block on 8-bit products: takes and returns the last branch's output and the stream that it is still to be added to."""
+        B, T, C = x.shape
+        dtype = fused_ops._compute_dtype(x)
+        h, x = _norm_of_sum(branch, x, self.attn_norm)
+        shape = (B, T, self.n_head, C // self.n_head)
+        q, k, v = (t.view(shape).transpose(1, 2) for t in self._fp8(h, dtype, "wq", "wk", "wv"))
+        a = F.scaled_dot_product_attention(_apply_rope(q, cos, sin), _apply_rope(k, cos, sin), v, is_causal=True)
+        (branch,) = self._fp8(a.transpose(1, 2).reshape(B, T, C), dtype, "wo")
+        h, x = _norm_of_sum(branch.view(x.shape), x, self.ffn_norm)
+        gate, up = self._fp8(h, dtype, "w_gate", "w_up")
+        (branch,) = self._fp8(F.silu(gate) * up, dtype, "w_down")
+        return branch.view(x.shape), x
+
+
+def _norm_of_sum(branch: torch.Tensor | None, x: torch.Tensor, norm: RMSNorm):
+    """``x + branch`` and its RMSNorm: ``(normalised, sum)``; the normalised rows come in 8 bits where no gradient is wanted."""
+    if not torch.is_grad_enabled():
+        return fp8.add_rms_norm(x, None, norm.weight, norm.eps) if branch is None else fp8.add_rms_norm(branch, x, norm.weight, norm.eps)
+    if branch is None:
+        return fused_ops.rms_norm(x, norm.weight, norm.eps), x
+    return fused_ops.add_rms_norm(branch, x, norm.weight, norm.eps)
+
 
 class Llama(nn.Module):
     def __init__(self, cfg: LlamaConfig | None = None) -> None:
@@ -94,15 +128,35 @@ class Llama(nn.Module):
             if isinstance(m, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(m.weight, mean=0.0, std=0.02)
 
+    def hold_fp8_weights(self) -> None:
+        """Keep the blocks' weights in 8 bits for calls without gradients, until ``train()``; a weight that changes meanwhile needs a new call."""
+        if not self.cfg.fp8:
+            raise ValueError("hold_fp8_weights needs a model with fp8=True")
+        for layer in self.layers:
+            layer._held = {n: fp8.quantize_weight(getattr(layer, n).weight) for n in layer._LINEARS}
+
+    def train(self, mode: bool = True):
+        if mode:
+            for layer in self.layers:
+                layer._held = None
+        return super().train(mode)
+
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         T = idx.shape[1]
         cos, sin = _rope_tables(T, self.cfg.d_model // self.cfg.n_head, self.cfg.rope_theta, idx.device)
-        x = self.embed(idx)
-        for layer in self.layers:
-            x = layer(x, cos, sin)
+        x = fused_ops.embedding(idx, self.embed.weight) if self.cfg.fused_embedding else self.embed(idx)
+        if self.cfg.fp8:
+            branch = None
+            for layer in self.layers:
+                branch, x = layer.forward_fp8(branch, x, cos, sin)
+            h = self.norm(x) if branch is None else fused_ops.add_rms_norm(branch, x, self.norm.weight, self.norm.eps)[0]
+        else:
+            for layer in self.layers:
+                x = layer(x, cos, sin)
+            h = self.norm(x)
         if self.cfg.fused and targets is not None:
-            return fused_ops.lm_head_cross_entropy(self.norm(x), self.head.weight, targets)
-        logits = self.head(self.norm(x))
+            return fused_ops.lm_head_cross_entropy(h, self.head.weight, targets)
+        logits = self.head(h)
         if targets is None:
             return logits
         return F.cross_entropy(logits.view(-1, logits.size(-1)).float(), targets.reshape(-1))

@@ -23,6 +23,7 @@
 #include "eig_kernels.cuh"
 #include "flat_kernels.cuh"
 #include "grouped_gemm.cuh"
+#include "tensor_map.h"
 #include "two_sided_apply.h"
 
 namespace py = pybind11;
@@ -30,25 +31,13 @@ using namespace ob200;
 
 namespace ob200 {
 void register_model_ops(pybind11::module_& m);  // model_kernels.cu
+void register_clip_ops(pybind11::module_& m);   // clip_kernels.cu
+void register_embed_ops(pybind11::module_& m);  // embed_kernels.cu
+void register_residual_norm_ops(pybind11::module_& m);  // residual_norm.cu
+void register_fp8_ops(pybind11::module_& m);    // fp8_kernels.cu
 }
 
 namespace {
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn get_encode_fn() {
-  static EncodeFn fn = nullptr;
-  if (fn == nullptr) {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    cudaError_t err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres);
-    TORCH_CHECK(err == cudaSuccess && sym != nullptr, "cuTensorMapEncodeTiled is not available from the driver");
-    fn = reinterpret_cast<EncodeFn>(sym);
-  }
-  return fn;
-}
 
 // Tensor map of a K-major fp32 operand: `t` is a 2-D view [rows, K] whose last stride is 1.
 CUtensorMap encode_operand(const torch::Tensor& t, int box_rows) {
@@ -1671,4 +1660,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("build_copy_table", &build_copy_table);
   m.def("peer_copy", &peer_copy);
   ob200::register_model_ops(m);
+  ob200::register_clip_ops(m);
+  ob200::register_embed_ops(m);
+  ob200::register_residual_norm_ops(m);
+  ob200::register_fp8_ops(m);
 }
