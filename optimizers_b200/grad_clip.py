@@ -138,7 +138,13 @@ def clip_grad_norm_(
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f"Invalid max_norm: {max_norm}")
-    parameters = parameters if isinstance(parameters, Tensor) else list(parameters)
+    parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    if shard_group is None and not error_if_nonfinite and parameters and getattr(parameters[0], "is_cuda", False):
+        from optimizers_b200.ops import build
+
+        norm = build.load().clip_parameters(parameters, max_norm)
+        if norm is not None:
+            return norm
     grads = _gradients(parameters, shard_group)
     if not grads:
         return _no_gradients(parameters, shard_group)

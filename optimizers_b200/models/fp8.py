@@ -147,17 +147,20 @@ def _squares(w: Tensor, transpose: bool, native: bool) -> tuple[tuple[Tensor, Te
     return (_e4m3(raw, w.shape[1]), scale), (_e4m3(raw_t, w.shape[0]), scale.t()) if transpose else None
 
 
-def _product(a, b, column_scales: bool, dtype: torch.dtype, native: bool, addend: Tensor | None = None) -> Tensor:
+def _product(a, b, column_scales: bool, dtype: torch.dtype, native: bool, addend: Tensor | None = None, shape=None) -> Tensor:
     """``a @ b.T`` (+ addend, fp32) in ``dtype``; b has a scale per row (``column_scales``) or per 128 rows."""
-    if native:
-        out = fused_ops._ext().fp8_matmul(
-            a[0].view(torch.uint8), a[1], b[0].view(torch.uint8), b[1], column_scales, dtype == torch.bfloat16, addend, _status_of(a[0].device)
-        )
-        fused_ops._count()
-        return out
+    if not native:
+        return _plain_product(a, b, 1 if column_scales else GROUP, dtype)
+    out = fused_ops._ext().fp8_matmul(
+        a[0].view(torch.uint8), a[1], b[0].view(torch.uint8), b[1], column_scales, dtype == torch.bfloat16, addend, _status_of(a[0].device), shape
+    )
+    fused_ops._count()
+    return out
+
+
+def _plain_product(a, b, down: int, dtype: torch.dtype) -> Tensor:
     with torch.autocast(a[0].device.type, enabled=False):
-        out = _values(*a, 1) @ _values(*b, 1 if column_scales else GROUP).t()
-    return (out if addend is None else out + addend).to(dtype)
+        return (_values(*a, 1) @ _values(*b, down).t()).to(dtype)
 
 
 def _aligned(data: Tensor) -> Tensor:
@@ -174,13 +177,21 @@ def _aligned(data: Tensor) -> Tensor:
 # Public functions
 # --------------------------------------------------------------------------------------------------
 def _is_native(x: Tensor) -> bool:
-    return fused_ops._native(x) and x.numel() > 0
+    return fused_ops._kernels_take(x) and x.numel() > 0
+
+
+def _rows_of(data: Tensor, scale: Tensor) -> Rows:
+    """Rows without the checks, for results of the kernels."""
+    rows = object.__new__(Rows)
+    object.__setattr__(rows, "data", data)
+    object.__setattr__(rows, "scale", scale)
+    return rows
 
 
 def quantize_rows(x: Tensor) -> Rows:
     """``x`` [..., K] in 8 bits as [T, K], a scale per 128 columns of each row (no gradient)."""
     x2 = x.detach().reshape(-1, x.shape[-1])
-    return Rows(*_rows(x2, _is_native(x2) and x2.dtype in _SOURCES))
+    return Rows(*_rows(x2, _is_native(x2)))
 
 
 def quantize_weight(weight: Tensor) -> Weight:
@@ -188,17 +199,21 @@ def quantize_weight(weight: Tensor) -> Weight:
     if weight.dim() != 2:
         raise ValueError(f"a weight is a matrix, got shape {tuple(weight.shape)}")
     w = weight.detach()
-    return Weight(*_squares(w, False, _is_native(w) and w.dtype in _SOURCES)[0])
+    return Weight(*_squares(w, False, _is_native(w))[0])
 
 
 @torch.no_grad()
 def _norm_rows(x: Tensor, residual: Tensor | None, weight: Tensor, eps: float) -> tuple[Rows, Tensor]:
     C = x.shape[-1]
-    x2, r2 = fused_ops._norm_operands(x, residual)
-    if fused_ops._add_norm_native(x2, r2, weight):
-        raw, scale, h, _ = fused_ops._ext().add_norm_fwd(x2, r2, weight.contiguous(), eps, 2, False)
+    given = (x, weight) if residual is None else (x, weight, residual)
+    if fused_ops._kernels_take(*given) and 0 < C <= fused_ops._MOST_COLUMNS and x.numel() > 0:
+        if residual is not None and x.dtype == torch.float32 and residual.dtype == torch.bfloat16:
+            residual = residual.float()  # an fp32 x is added to a residual in fp32
+        raw, scale, h, _ = fused_ops._ext().add_norm_fwd(
+            x.contiguous(), None if residual is None else residual.contiguous(), weight.contiguous(), eps, 2, False
+        )
         fused_ops._count()
-        return Rows(_e4m3(raw, C), scale.t()), (x if residual is None else h.view(x.shape))
+        return _rows_of(_e4m3(raw, C), scale.t()), (x if residual is None else h)
     h = x if residual is None else (x.float() + residual.float()).to(torch.promote_types(x.dtype, residual.dtype))
     hf = h.float().reshape(-1, C)
     y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
@@ -215,40 +230,32 @@ def add_rms_norm(x: Tensor, residual: Tensor | None, weight: Tensor, eps: float 
 
 
 class _Linear(torch.autograd.Function):
+    """The plain form of the layer; the kernels' is a node of the extension."""
+
     @staticmethod
-    def forward(ctx, x: Tensor, dtype: torch.dtype, native: bool, *weights: Tensor):  # type: ignore[override]
-        need_dx, need_dw = ctx.needs_input_grad[0], any(ctx.needs_input_grad[3:])
-        rows, columns = _both(x, native) if need_dw else (_rows(x, native), None)
-        saved, out = [], []
-        for w in weights:
-            straight, turned = _squares(w, need_dx, native)
-            out.append(_product(rows, straight, False, dtype, native))
-            saved += list(turned) if need_dx else []
-        ctx.save_for_backward(*(columns or ()), *saved)
-        ctx.meta = (need_dw, need_dx, native, x.shape, x.dtype, [(w.shape, w.dtype) for w in weights])
+    def forward(ctx, x: Tensor, dtype: torch.dtype, *weights: Tensor):  # type: ignore[override]
+        rows = _plain_groups(x, 1)
+        squares = [_plain_groups(w, GROUP) for w in weights]
+        ctx.save_for_backward(*_plain_groups(x.t(), 1), *(t for sq in squares for t in sq))
+        ctx.meta = (x.dtype, [w.dtype for w in weights])
         ctx.set_materialize_grads(False)
-        return tuple(out)
+        return tuple(_plain_product(rows, sq, GROUP, dtype) for sq in squares)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):  # type: ignore[override]
-        need_dw, need_dx, native, x_shape, x_dtype, metas = ctx.meta
-        saved = list(ctx.saved_tensors)
-        columns = (saved.pop(0), saved.pop(0)) if need_dw else None
-        live = [i for i, dy in enumerate(grads) if dy is not None]
-        dx, dws = None, [None] * len(metas)
-        for i in live:
-            dy = grads[i]
-            if dy.dtype not in _SOURCES:
-                dy = dy.float()
-            want_dw = ctx.needs_input_grad[3 + i]
-            across, down = _both(dy, native) if want_dw else (_rows(dy, native) if need_dx else None, None)
-            if need_dx:
-                last = i == live[-1]  # sums over several layers stay in 32 bits until then
-                dx = _product(across, (saved[2 * i], saved[2 * i + 1]), False, x_dtype if last else torch.float32, native, dx)
-            if want_dw:
-                dws[i] = _product(down, columns, True, metas[i][1], native)
-        return (dx, None, None, *dws)
+        x_dtype, w_dtypes = ctx.meta
+        saved = ctx.saved_tensors
+        dx, dws = None, [None] * len(w_dtypes)
+        for i, dy in enumerate(grads):
+            if dy is None:
+                continue
+            if ctx.needs_input_grad[0]:  # sums over several layers stay in 32 bits
+                part = _plain_product(_plain_groups(dy, 1), (saved[2 + 2 * i].t(), saved[3 + 2 * i].t()), GROUP, torch.float32)
+                dx = part if dx is None else dx + part
+            if ctx.needs_input_grad[2 + i]:
+                dws[i] = _plain_product(_plain_groups(dy.t(), 1), saved[:2], 1, w_dtypes[i])
+        return (None if dx is None else dx.to(x_dtype), None, *dws)
 
 
 def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight], out_dtype: torch.dtype | None = None):
@@ -263,37 +270,41 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
         raise ValueError("linear needs a weight")
     held_x = isinstance(x, Rows)
     source = x.data if held_x else x
+    tensors, empty = [], source.numel() == 0
     for w in weights:
-        shape = w.data.shape if isinstance(w, Weight) else w.shape
-        if len(shape) != 2 or shape[1] != source.shape[-1]:
-            raise ValueError(f"a weight of shape {tuple(shape)} does not fit rows of {source.shape[-1]}")
-        if (w.data if isinstance(w, Weight) else w).device != source.device:
-            raise ValueError(f"weight on {w.data.device}, x on {source.device}")
+        held = isinstance(w, Weight)
+        data = w.data if held else w
+        if data.dim() != 2 or source.dim() < 1 or data.shape[1] != source.shape[-1]:
+            raise ValueError(f"a weight of shape {tuple(data.shape)} does not fit rows of shape {tuple(source.shape)}")
+        if data.device != source.device:
+            raise ValueError(f"weight on {data.device}, x on {source.device}")
+        empty = empty or data.numel() == 0
+        if not held:
+            tensors.append(w)
     if out_dtype is None:
         out_dtype = torch.bfloat16 if held_x else fused_ops._compute_dtype(x)
     if not out_dtype.is_floating_point or (not held_x and not x.is_floating_point()):
         raise ValueError("linear takes and returns floating-point tensors")
-    tensors = [w for w in weights if isinstance(w, Tensor)]
-    learns = torch.is_grad_enabled() and (any(w.requires_grad for w in tensors) or (not held_x and x.requires_grad))
-    empty = source.numel() == 0 or any((w.data if isinstance(w, Weight) else w).numel() == 0 for w in weights)
-    native = (
-        fused_ops._native(source) and not empty and out_dtype in _SOURCES and (held_x or x.dtype in _SOURCES)
-        and all(w.dtype in _SOURCES for w in tensors)
-    )
-    if learns:
+    operands = tensors if held_x else [x, *tensors]
+    native = not empty and out_dtype in _SOURCES and (fused_ops._kernels_take(*operands) if operands else fused_ops._native(source))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         if held_x or len(tensors) < len(weights):
             raise ValueError("operands held in 8 bits carry no gradient: pass tensors for x and every weight in training, or use torch.no_grad()")
-        out = _Linear.apply(x.reshape(-1, x.shape[-1]), out_dtype, native, *weights)
-        out = tuple(y.view(*x.shape[:-1], y.shape[-1]) for y in out)
+        if native:
+            out = fused_ops._ext().fp8_linear(x, tensors, out_dtype == torch.bfloat16, _status_of(x.device))
+        else:
+            out = _Linear.apply(x.reshape(-1, x.shape[-1]), out_dtype, *tensors)
+            out = [y.view(*x.shape[:-1], y.shape[-1]) for y in out]
     else:
-        with torch.no_grad():
-            rows = (x.data, x.scale) if held_x else _rows(x.reshape(-1, x.shape[-1]), native)
-            if native and held_x:
-                rows = (_aligned(rows[0]), rows[1])
-            shape = x.data.shape[:1] if held_x else x.shape[:-1]
-            out = []
-            for w in weights:
-                held = _squares(w, False, native)[0] if isinstance(w, Tensor) else (_aligned(w.data) if native else w.data, w.scale)
-                out.append(_product(rows, held, False, out_dtype, native).view(*shape, held[0].shape[0]))
-            out = tuple(out)
-    return out if several else out[0]
+        rows = (x.data, x.scale) if held_x else _rows(x.detach().reshape(-1, x.shape[-1]), native)
+        if native and held_x:
+            rows = (_aligned(rows[0]), rows[1])
+        out = []
+        for w in weights:
+            if isinstance(w, Weight):
+                held = (_aligned(w.data) if native else w.data, w.scale)
+            else:
+                held = _squares(w.detach(), False, native)[0]
+            shape = [*source.shape[:-1], held[0].shape[0]]
+            out.append(_product(rows, held, False, out_dtype, native, shape=shape) if native else _product(rows, held, False, out_dtype, False).view(shape))
+    return tuple(out) if several else out[0]

@@ -37,7 +37,6 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 _ENABLED = True
 _EXT = None
@@ -198,32 +197,6 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
 # --------------------------------------------------------------------------------------------------
 # Residual addition + RMSNorm
 # --------------------------------------------------------------------------------------------------
-class _AddNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, residual: Tensor, weight: Tensor, eps: float, out_dtype: torch.dtype):  # type: ignore[override]
-        w = weight.contiguous()
-        y, _, h, rstd = _ext().add_norm_fwd(x, residual, w, eps, 1 if out_dtype == torch.bfloat16 else 0, True)
-        _count()
-        ctx.save_for_backward(h, w, rstd)
-        ctx.x_dtype = x.dtype
-        ctx.set_materialize_grads(False)
-        return y, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy: Tensor | None, dh: Tensor | None):  # type: ignore[override]
-        h, w, rstd = ctx.saved_tensors
-        if dy is None:  # only the sum was used
-            return (None if dh is None else dh.to(ctx.x_dtype)), dh, (torch.zeros_like(w) if dh is not None else None), None, None
-        if dy.dtype not in (torch.float32, torch.bfloat16):
-            dy = dy.float()
-        dx, dr, dw = _ext().add_norm_bwd(
-            dy.contiguous(), None if dh is None else dh.contiguous(), h, w, rstd, ctx.x_dtype == torch.bfloat16, True
-        )
-        _count()
-        return dx, dr, dw, None, None
-
-
 def _check_add_norm(x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
     if x.dim() < 1 or weight.shape != x.shape[-1:]:
         raise ValueError(f"a norm weight of shape {tuple(weight.shape)} does not fit rows of shape {tuple(x.shape)}")
@@ -233,22 +206,30 @@ def _check_add_norm(x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
         raise ValueError("add_rms_norm takes floating-point tensors")
 
 
-def _norm_operands(x: Tensor, residual: Tensor | None) -> tuple[Tensor, Tensor | None]:
-    """Contiguous rows; an fp32 x is added to a residual in fp32."""
-    x2 = x.reshape(-1, x.shape[-1]).contiguous()
-    if residual is None:
-        return x2, None
-    if x.dtype == torch.float32 and residual.dtype == torch.bfloat16:
-        residual = residual.float()
-    return x2, residual.reshape(x2.shape).contiguous()
+_MOST_COLUMNS = 16384  # of a row that the kernels take
+_KINDS = (torch.float32, torch.bfloat16)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_on_sm100: dict[int | None, bool] = {}
 
 
-def _add_norm_native(x2: Tensor, r2: Tensor | None, weight: Tensor) -> bool:
-    kinds = (torch.float32, torch.bfloat16)
-    return (
-        _native(x2) and x2.numel() > 0 and x2.dtype in kinds and weight.dtype in kinds and weight.device == x2.device
-        and (r2 is None or (r2.dtype in kinds and r2.device == x2.device)) and x2.shape[1] <= _ext().add_norm_max_width()
-    )
+def _kernels_take(*tensors: Tensor) -> bool:
+    """Whether the kernels read these: plain fp32 or bf16 tensors on one sm_100 device."""
+    first = tensors[0]
+    if not (_ENABLED and first.is_cuda):
+        return False
+    device = first.device
+    known = _on_sm100.get(device.index)
+    if known is None:
+        known = _on_sm100[device.index] = torch.cuda.get_device_capability(device)[0] == 10
+    for t in tensors:
+        if t.dtype not in _KINDS or type(t) not in _PLAIN or t.device != device:
+            return False
+    return known
+
+
+def launches() -> int:
+    """Kernels of the model operations launched so far by this process, backward passes included."""
+    return launch_count + (_EXT.model_op_launches() if _EXT is not None else 0)
 
 
 def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
@@ -258,10 +239,8 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6)
         raise ValueError("add_rms_norm needs a residual; rms_norm normalises x alone")
     _check_add_norm(x, residual, weight)
     out_dtype = _norm_out_dtype(x)
-    x2, r2 = _norm_operands(x, residual)
-    if _add_norm_native(x2, r2, weight):
-        y, h = _AddNorm.apply(x2, r2, weight, eps, out_dtype)
-        return y.view(x.shape), h.view(x.shape)
+    if _kernels_take(x, residual, weight) and 0 < x.shape[-1] <= _MOST_COLUMNS and x.numel() > 0:
+        return _ext().add_rms_norm(x, residual, weight, eps, out_dtype == torch.bfloat16)
     h = (x.float() + residual.float()).to(torch.promote_types(x.dtype, residual.dtype))
     hf = h.float()
     y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps)
@@ -271,26 +250,6 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6)
 # --------------------------------------------------------------------------------------------------
 # Token embedding
 # --------------------------------------------------------------------------------------------------
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids: Tensor, weight: Tensor, scale: float, out_dtype: torch.dtype):  # type: ignore[override]
-        ctx.save_for_backward(ids)
-        ctx.meta = (weight.shape[0], scale, weight.dtype)
-        y = _ext().embed_fwd(ids, weight.contiguous(), scale, out_dtype == torch.bfloat16)
-        _count()
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy: Tensor):  # type: ignore[override]
-        (ids,) = ctx.saved_tensors
-        rows, scale, dtype = ctx.meta
-        dy = dy.contiguous() if dy.dtype in (torch.float32, torch.bfloat16) else dy.float().contiguous()
-        dw = _ext().embed_bwd(ids, dy, rows, scale, dtype == torch.bfloat16)
-        _count()
-        return None, dw, None, None
-
-
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> Tensor:
     """``scale * weight[ids]`` in ``out_dtype`` (the table's by default), for integer ``ids`` of any shape and a table [V, C].
 
@@ -305,9 +264,8 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     if not (weight.is_floating_point() and out_dtype.is_floating_point):
         raise ValueError("embedding takes and returns floating-point tensors")
-    kinds = (torch.float32, torch.bfloat16)
-    if _native(weight) and ids.device == weight.device and weight.dtype in kinds and out_dtype in kinds and weight.numel() > 0:
-        return _Embedding.apply(ids.reshape(-1).contiguous(), weight, float(scale), out_dtype).view(*ids.shape, weight.shape[1])
+    if _kernels_take(weight) and type(ids) is torch.Tensor and ids.device == weight.device and out_dtype in _KINDS and weight.numel() > 0:
+        return _ext().embedding(ids, weight, scale, out_dtype == torch.bfloat16)
     y = F.embedding(ids, weight)
     return y.to(out_dtype) if scale == 1.0 else (y.float() * scale).to(out_dtype)
 

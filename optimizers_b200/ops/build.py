@@ -22,7 +22,7 @@ _SO = _HERE / f"{_NAME}.so"
 _module: ModuleType | None = None
 
 SOURCES = ["bindings.cu", "grouped_gemm.cu", "block_kernels.cu", "flat_kernels.cu", "eig_kernels.cu", "two_sided_apply.cu", "model_kernels.cu",
-           "clip_kernels.cu", "embed_kernels.cu", "residual_norm.cu", "fp8_kernels.cu"]
+           "clip_kernels.cu", "embed_kernels.cu", "residual_norm.cu", "fp8_kernels.cu", "model_autograd.cpp"]
 NVCC_FLAGS = [
     "-gencode",
     "arch=compute_100a,code=sm_100a",
@@ -37,7 +37,7 @@ def _stale() -> bool:
     if not _SO.exists():
         return True
     built = _SO.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in _CSRC.iterdir() if p.suffix in (".cu", ".cuh", ".h"))
+    return any(p.stat().st_mtime > built for p in _CSRC.iterdir() if p.suffix in (".cu", ".cuh", ".h", ".cpp"))
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

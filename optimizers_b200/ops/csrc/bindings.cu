@@ -35,6 +35,7 @@ void register_clip_ops(pybind11::module_& m);   // clip_kernels.cu
 void register_embed_ops(pybind11::module_& m);  // embed_kernels.cu
 void register_residual_norm_ops(pybind11::module_& m);  // residual_norm.cu
 void register_fp8_ops(pybind11::module_& m);    // fp8_kernels.cu
+void register_model_autograd(pybind11::module_& m);  // model_autograd.cpp
 }
 
 namespace {
@@ -1664,4 +1665,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   ob200::register_embed_ops(m);
   ob200::register_residual_norm_ops(m);
   ob200::register_fp8_ops(m);
+  ob200::register_model_autograd(m);
 }

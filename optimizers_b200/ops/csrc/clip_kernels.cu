@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <unordered_set>
 
 namespace ob200 {
 namespace {
@@ -306,9 +307,31 @@ torch::Tensor clip_scale(const std::vector<torch::Tensor>& grads, const torch::T
   return norm;
 }
 
+// The whole call for the usual case, without a pass over the gradients in Python: every gradient on one sm_100 device, of these
+// types, filling its memory.  None otherwise, and where there is no gradient.
+std::optional<torch::Tensor> clip_parameters(const std::vector<torch::Tensor>& parameters, double max_norm) {
+  std::vector<torch::Tensor> grads;
+  std::unordered_set<const void*> seen;
+  grads.reserve(parameters.size());
+  for (const auto& p : parameters) {
+    if (!p.defined() || !p.is_leaf()) return std::nullopt;
+    const auto& g = p.grad();
+    if (!g.defined() || !seen.insert(p.unsafeGetTensorImpl()).second) continue;
+    const auto st = g.scalar_type();
+    if (g.unsafeGetTensorImpl()->is_python_dispatch() || g.layout() != torch::kStrided || !g.is_cuda() ||
+        (st != torch::kFloat32 && st != torch::kBFloat16 && st != torch::kFloat16) || !g.is_non_overlapping_and_dense() ||
+        (!grads.empty() && g.device() != grads[0].device()))
+      return std::nullopt;
+    grads.push_back(g);
+  }
+  if (grads.empty() || at::cuda::getDeviceProperties(grads[0].device().index())->major != 10) return std::nullopt;
+  return clip_scale(grads, grad_sumsq(grads, true), max_norm);
+}
+
 void register_clip_ops(pybind11::module_& m) {
   m.def("grad_sumsq", &grad_sumsq);
   m.def("clip_scale", &clip_scale);
+  m.def("clip_parameters", &clip_parameters);
 }
 
 }  // namespace ob200

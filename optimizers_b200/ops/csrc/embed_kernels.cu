@@ -103,7 +103,13 @@ embed_sort_kernel(const Id* __restrict__ ids, int n, long long V, int bits, unsi
   if (blockIdx.x >= kSortCtas) {  // the zeros of the table
     const long long stride = static_cast<long long>(gridDim.x - kSortCtas) * kSortThreads;
     const long long t = static_cast<long long>(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
-    for (long long i = t; i < zero_vecs; i += stride) __stcs(zero + i, make_uint4(0u, 0u, 0u, 0u));
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    long long i = t;
+    for (; i + 7 * stride < zero_vecs; i += 8 * stride) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) zero[i + q * stride] = none;
+    }
+    for (; i < zero_vecs; i += stride) zero[i] = none;
     if (t < tail_bytes) zero_tail[t] = 0;
     return;
   }
@@ -319,20 +325,22 @@ void with_ids(const torch::Tensor& ids, F&& f) {
 }
 
 void check_ids(const torch::Tensor& ids, const torch::Tensor& other) {
-  TORCH_CHECK(ids.is_cuda() && ids.device() == other.device() && ids.dim() == 1 && ids.is_contiguous() &&
-                  (ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32), "embedding: ids are contiguous int64 or int32 [n] on the table's device");
+  TORCH_CHECK(ids.is_cuda() && ids.device() == other.device() && ids.is_contiguous() &&
+                  (ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32), "embedding: ids are contiguous int64 or int32 on the table's device");
 }
 
 }  // namespace
 
-// ids [n], table [V, C] -> [n, C]
+// ids [...], table [V, C] -> [..., C]
 torch::Tensor embed_fwd(const torch::Tensor& ids, const torch::Tensor& table, double scale, bool out_bf16) {
   TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.is_contiguous() && fp32_or_bf16(table), "embedding: the table is contiguous fp32 or bf16 [V, C]");
   check_ids(ids, table);
   const int64_t n = ids.numel(), V = table.size(0), C = table.size(1);
   TORCH_CHECK(V > 0 && V < (1LL << 31) && C < (1LL << 31), "embedding: table size");
   c10::cuda::CUDAGuard guard(table.device());
-  auto out = torch::empty({n, C}, table.options().dtype(out_bf16 ? torch::kBFloat16 : torch::kFloat32));
+  auto sizes = ids.sizes().vec();
+  sizes.push_back(C);
+  auto out = torch::empty(sizes, table.options().dtype(out_bf16 ? torch::kBFloat16 : torch::kFloat32));
   if (out.numel() == 0) return out;
   auto st = at::cuda::getCurrentCUDAStream();
   const int N = table.scalar_type() == torch::kFloat32 && !out_bf16 ? 4 : 8;
@@ -358,11 +366,12 @@ torch::Tensor embed_fwd(const torch::Tensor& ids, const torch::Tensor& table, do
   return out;
 }
 
-// ids [n], dy [n, C] -> gradient of the table [V, C], fp32 or bf16
+// ids [...], dy [..., C] -> gradient of the table [V, C], fp32 or bf16
 torch::Tensor embed_bwd(const torch::Tensor& ids, const torch::Tensor& dy, int64_t V, double scale, bool out_bf16) {
-  TORCH_CHECK(dy.is_cuda() && dy.dim() == 2 && dy.is_contiguous() && fp32_or_bf16(dy) && dy.size(0) == ids.numel(), "embedding: dy is contiguous fp32 or bf16 [n, C]");
+  TORCH_CHECK(dy.is_cuda() && dy.dim() == ids.dim() + 1 && dy.is_contiguous() && fp32_or_bf16(dy) && dy.numel() == ids.numel() * dy.size(-1),
+              "embedding: dy is contiguous fp32 or bf16 [..., C]");
   check_ids(ids, dy);
-  const int64_t n = ids.numel(), C = dy.size(1);
+  const int64_t n = ids.numel(), C = dy.size(-1);
   TORCH_CHECK(V > 0 && V < (1LL << 31) && C < (1LL << 31), "embedding: table size");
   c10::cuda::CUDAGuard guard(dy.device());
   // Batches beyond the sort's capacity are taken in slices that add to the table, in fp32 whatever the result's type.

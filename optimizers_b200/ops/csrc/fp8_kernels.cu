@@ -6,11 +6,17 @@
 //   fp8_matmul    C[m, n] = sum_g sa[m, g] sb[n, g] sum_{k in g} a[m, k] b[n, k]
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cooperative_groups.h>
 #include <torch/extension.h>
+
+#include <mutex>
+#include <set>
 
 #include "fp8_format.cuh"
 #include "ptx.cuh"
 #include "tensor_map.h"
+
+namespace cg = cooperative_groups;
 
 namespace ob200 {
 namespace {
@@ -21,47 +27,98 @@ using bf16 = __nv_bfloat16;
 // Into the format.  Bound by HBM: one read of x, one byte written per value and operand.
 // ------------------------------------------------------------------------------------------------
 constexpr int kRowsThreads = 256;
+constexpr int kRowsAtOnce = 4;  // groups of sixteen lanes in flight
 
-// Sixteen lanes take one group, eight values each.
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, magnitude_bits(v[k]));
+  return top;
+}
+
+// Largest of each of kCount values over sixteen lanes, a value per lane at the end: lane l holds that of number l * kCount / 16.  One division
+// per lane then serves all groups.
+template <int kCount>
+__device__ __forceinline__ uint32_t spread_max(uint32_t (&v)[kCount], int lane) {
+  int o = 8;
+#pragma unroll
+  for (int n = kCount; n > 1; n >>= 1, o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const bool high = lane & o;
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + n / 2], o);
+      v[i] = max(high ? v[i + n / 2] : v[i], got);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) v[0] = max(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+  return v[0];
+}
+
+// Sixteen lanes take four groups, eight values each of every group.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale, long long rows, int K) {
   const int groups = (K + kFp8Group - 1) / kFp8Group, lane = threadIdx.x & 15;
   const long long total = rows * groups;
-  const long long g = (static_cast<long long>(blockIdx.x) * kRowsThreads + threadIdx.x) >> 4;
-  const long long row = g < total ? g / groups : 0;
-  const int kb = g < total ? static_cast<int>(g % groups) : 0;
-  const int col = kb * kFp8Group + lane * 8;
-  float v[8];
-  load8<kVec>(x + row * ldx, col, K, v);
-  uint32_t top = 0;
+  const long long first = ((static_cast<long long>(blockIdx.x) * kRowsThreads + threadIdx.x) >> 4) * kRowsAtOnce;
+  float v[kRowsAtOnce][8];
+  long long row = first / groups;
+  int kb = static_cast<int>(first - row * groups);
+  const long long row0 = row;
+  const int kb0 = kb;
+  uint32_t top[kRowsAtOnce];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = max(top, magnitude_bits(v[k]));
+  for (int i = 0; i < kRowsAtOnce; ++i) {
+    if (first + i < total) {
+      load8<kVec>(x + row * ldx, kb * kFp8Group + lane * 8, K, v[i]);
+    } else {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (g >= total) return;
-  const GroupScale s = group_scale(top);
-  if (col < K) *reinterpret_cast<uint2*>(q + row * ldq + col) = e4m3x8(v, s.factor);  // the pitch is a multiple of 16
-  if (lane == 0) scale[static_cast<long long>(kb) * rows + row] = s.scale;
+      for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
+    }
+    if (++kb == groups) {
+      kb = 0;
+      ++row;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRowsAtOnce; ++i) top[i] = top_of(v[i]);
+  const GroupScale s = group_scale(spread_max(top, lane));
+  row = row0;
+  kb = kb0;
+#pragma unroll
+  for (int i = 0; i < kRowsAtOnce; ++i) {
+    const int from = (threadIdx.x & 16) + i * (16 / kRowsAtOnce);
+    const float factor = __shfl_sync(0xffffffffu, s.factor, from), held = __shfl_sync(0xffffffffu, s.scale, from);
+    if (first + i < total) {
+      const int col = kb * kFp8Group + lane * 8;
+      if (col < K) *reinterpret_cast<uint2*>(q + row * ldq + col) = e4m3x8(v[i], factor);  // the pitch is a multiple of 16
+      if (lane == 0) scale[static_cast<long long>(kb) * rows + row] = held;
+    }
+    if (++kb == groups) {
+      kb = 0;
+      ++row;
+    }
+  }
 }
 
 // A CTA takes a 128 x 128 tile: thread (ty, tx) holds rows 8 ty .. 8 ty + 7 and columns 8 tx .. 8 tx + 7.  The transpose goes through
-// shared memory, where a thread has eight neighbouring bytes of each of its columns.
+// shared memory, where a thread has eight neighbouring bytes of each of its columns; piece p of row c lies at p ^ (c / 8), so that the
+// threads of a row of tiles write to different banks.
 constexpr int kTileThreads = 256;
-constexpr int kTilePitch = 128 + 16;  // bytes
 
 template <typename T, bool kVec, bool kSquares>
-__global__ void __launch_bounds__(kTileThreads)
+__global__ void __launch_bounds__(kTileThreads, 2)
 fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale, uint8_t* __restrict__ qt,
                 long long ldt, float* __restrict__ scale_t, long long rows, int K) {
-  __shared__ uint32_t col_top[kFp8Group];
-  __shared__ __align__(16) uint8_t flipped[kFp8Group * kTilePitch];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  __shared__ __align__(16) uint32_t col_top[kTileThreads / 32][kFp8Group];
+  __shared__ __align__(16) float col_factor[kFp8Group];
+  __shared__ __align__(16) uint8_t flipped[kFp8Group * kFp8Group];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5;
   const int kb = blockIdx.x;
   const long long tb = blockIdx.y;
   const int col = kb * kFp8Group + tx * 8;
   const long long row0 = tb * kFp8Group + ty * 8;
-  if (threadIdx.x < kFp8Group) col_top[threadIdx.x] = 0;
   float v[8][8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
@@ -72,68 +129,77 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
       for (int k = 0; k < 8; ++k) v[r][k] = 0.f;
     }
   }
-  __syncthreads();
-  uint32_t tops[8];  // of a thread's columns
+  uint32_t tops[8];  // of a thread's rows
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    uint32_t t = 0;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) t = max(t, magnitude_bits(v[r][k]));
-    tops[k] = t;
-  }
+  for (int r = 0; r < 8; ++r) tops[r] = top_of(v[r]);
   float factor_t[8];
   if constexpr (kSquares) {
     uint32_t t = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t = max(t, tops[k]);
+    for (int r = 0; r < 8; ++r) t = max(t, tops[r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
-    if ((threadIdx.x & 31) == 0) atomicMax(&col_top[0], t);
+    if ((threadIdx.x & 31) == 0) col_top[0][warp] = t;
     __syncthreads();
-    const GroupScale s = group_scale(col_top[0]);
+    t = 0;
+#pragma unroll
+    for (int w = 0; w < kTileThreads / 32; ++w) t = max(t, col_top[0][w]);
+    const GroupScale s = group_scale(t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) factor_t[k] = s.factor;
     if (threadIdx.x == 0) scale[tb * gridDim.x + kb] = s.scale;
 #pragma unroll
     for (int r = 0; r < 8; ++r)
       if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = e4m3x8(v[r], s.factor);
+    if (qt == nullptr) return;
   } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) atomicMax(&col_top[tx * 8 + k], tops[k]);
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      uint32_t t = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) t = max(t, magnitude_bits(v[r][k]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
-      const GroupScale s = group_scale(t);
-      if (row0 + r < rows) {
-        if (col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = e4m3x8(v[r], s.factor);
-        if (tx == 0) scale[static_cast<long long>(kb) * rows + row0 + r] = s.scale;
-      }
-    }
-    __syncthreads();
+    uint32_t down[8];  // of a thread's columns, with the other eight rows of the warp
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const GroupScale s = group_scale(col_top[tx * 8 + k]);
-      factor_t[k] = s.factor;
-      if (ty == 0 && col + k < K) scale_t[tb * K + col + k] = s.scale;
+      uint32_t t = 0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) t = max(t, magnitude_bits(v[r][k]));
+      down[k] = max(t, __shfl_xor_sync(0xffffffffu, t, 16));
     }
+    if ((threadIdx.x & 16) == 0) {
+      *reinterpret_cast<uint4*>(&col_top[warp][tx * 8]) = make_uint4(down[0], down[1], down[2], down[3]);
+      *reinterpret_cast<uint4*>(&col_top[warp][tx * 8 + 4]) = make_uint4(down[4], down[5], down[6], down[7]);
+    }
+    const GroupScale mine = group_scale(spread_max(tops, tx));  // of row tx / 2
+    if ((tx & 1) == 0 && row0 + tx / 2 < rows) scale[static_cast<long long>(kb) * rows + row0 + tx / 2] = mine.scale;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float factor = __shfl_sync(0xffffffffu, mine.factor, (threadIdx.x & 16) + 2 * r);
+      if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = e4m3x8(v[r], factor);
+    }
+    __syncthreads();
+    if (threadIdx.x < kFp8Group) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int w = 0; w < kTileThreads / 32; ++w) t = max(t, col_top[w][threadIdx.x]);
+      const GroupScale s = group_scale(t);
+      col_factor[threadIdx.x] = s.factor;
+      if (kb * kFp8Group + threadIdx.x < K) scale_t[tb * K + kb * kFp8Group + threadIdx.x] = s.scale;
+    }
+    __syncthreads();
+    const float4 f0 = *reinterpret_cast<const float4*>(&col_factor[tx * 8]), f1 = *reinterpret_cast<const float4*>(&col_factor[tx * 8 + 4]);
+    factor_t[0] = f0.x; factor_t[1] = f0.y; factor_t[2] = f0.z; factor_t[3] = f0.w;
+    factor_t[4] = f1.x; factor_t[5] = f1.y; factor_t[6] = f1.z; factor_t[7] = f1.w;
   }
-  if (kSquares && qt == nullptr) return;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float c[8] = {v[0][k], v[1][k], v[2][k], v[3][k], v[4][k], v[5][k], v[6][k], v[7][k]};
-    *reinterpret_cast<uint2*>(flipped + (tx * 8 + k) * kTilePitch + ty * 8) = e4m3x8(c, factor_t[k]);
+    *reinterpret_cast<uint2*>(flipped + (tx * 8 + k) * kFp8Group + (ty ^ tx) * 8) = e4m3x8(c, factor_t[k]);
   }
   __syncthreads();
   // Row c of the transpose: 128 bytes, of which those beyond the pitch do not exist (the pitch is a multiple of 16).
   for (int i = threadIdx.x; i < kFp8Group * 8; i += kTileThreads) {
-    const int c = i >> 3, part = (i & 7) * 16;
-    if (kb * kFp8Group + c < K && tb * kFp8Group + part < ldt)
-      *reinterpret_cast<uint4*>(qt + static_cast<long long>(kb * kFp8Group + c) * ldt + tb * kFp8Group + part) =
-          *reinterpret_cast<const uint4*>(flipped + c * kTilePitch + part);
+    const int c = i >> 3, part = i & 7, turn = c >> 3;
+    if (kb * kFp8Group + c < K && tb * kFp8Group + part * 16 < ldt) {
+      const uint4 u = *reinterpret_cast<const uint4*>(flipped + c * kFp8Group + ((2 * part ^ turn) & ~1) * 8);
+      *reinterpret_cast<uint4*>(qt + static_cast<long long>(kb * kFp8Group + c) * ldt + tb * kFp8Group + part * 16) =
+          (turn & 1) ? make_uint4(u.z, u.w, u.x, u.y) : u;
+    }
   }
 }
 
@@ -141,20 +207,46 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
 // The product.  A tile of 128 x kN results goes over K in steps of one group of 128: TMA brings 128 x 128 bytes of A and kN x 128 of B,
 // four tcgen05.mma sum the group into a TMEM buffer of its own, and eight epilogue warps read the buffer, apply the two scales
 // of the group and add it to sums that stay in fp32 registers, while the MMAs of the next groups fill the other buffers.
+//
+// A thread of an epilogue warp holds one row where B has a scale per 128 rows: one multiply-add per value with the product of both
+// scales.  With a scale per row of B (a column of the tile) it holds every fourth column of four rows: two operations per value, but a
+// quarter of the scales to fetch from shared memory.  TMEM gives whole rows at 244 bytes per clock and 32 lanes, the latter
+// arrangement at 124 (column pairs of eight rows would come at 64); the fp32 units take one operation per clock.  So the epilogue needs about
+// 256 or 512 clocks per group of a 128 x 256 tile, next to 512 of the MMAs.  The next piece of a buffer is on its way while one is added.
+//
+// Large products are computed by pairs of CTAs, 256 x 256 results each: with 128 x 256 per CTA the loads from the L2 (48 KB per group and SM, 11.5
+// TB/s over the chip) bound the kernel at half of the tensor rate whatever the epilogue does; a pair loads 32 KB per group and SM.
+//
+// Products with few tiles are cut along K among the CTAs of a cluster, whose partial sums meet in distributed shared memory: each CTA adds
+// the sums of all ranks, in rank order, for its share of the tile.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTileM = 128;
 constexpr int kEpilogueWarps = 8;
-constexpr int kProductThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kFirstEpilogueWarp = 4;
+constexpr int kProductThreads = 384;  // warps 0 TMA, 1 and 2 MMA, one idle; 4 .. 11 epilogue
+constexpr int kMaxSplits = 8;
 
-template <int kN>
+template <int kN, bool kPair, bool kColumnScale, typename Out>
 struct ProductCfg {
-  static constexpr int kStageBytes = (kTileM + kN) * kFp8Group;
-  static constexpr int kStages = kN == 256 ? 4 : kN == 128 ? 6 : 8;
+  static constexpr int kRowsB = kPair ? kN / 2 : kN;  // that this CTA loads
+  static constexpr int kStageBytes = (kTileM + kRowsB) * kFp8Group;
   static constexpr int kBuffers = kN == 256 ? 2 : 4;  // TMEM buffers of kN columns
   static constexpr int kOwn = kN / 2;                 // columns of one epilogue warp: two warps share a 32-row stripe
-  static constexpr int kScaleFloats = kEpilogueWarps * kOwn;
-  static constexpr int kBarrierBytes = 256;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kScaleFloats * 4 + kBarrierBytes;  // 1 KB to align the stages
+  // Whole rows in bf16 leave through shared memory and TMA, 64 columns at a time.
+  static constexpr bool kStaged = sizeof(Out) == 2 && !kColumnScale && kN >= 128;
+  static constexpr int kStagingBytes = kStaged ? kEpilogueWarps * 32 * kOwn * 2 : 0;
+  static constexpr int kStages = kN == 64 ? 8 : kStaged ? 4 : 6;
+  static constexpr int kScaleSlots = 4;  // groups whose scales are on their way
+  static constexpr int kScaleFloats = kTileM + (kColumnScale ? kN : 32);             // of one group: rows of A, columns or blocks of B
+  static constexpr int kBarrierBytes = 320;
+  // 1 KB to align the stages
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kScaleSlots * kScaleFloats * 4 + kBarrierBytes;
+  // Registers: 128 sums per epilogue thread do not fit into an even split of 168, so the first warpgroup gives up some of its own.
+  static constexpr bool kUneven = kN == 256;
+  static constexpr int kLaunchRegs = 168, kEpilogueRegs = 232, kOtherRegs = 40;
+  static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kProductThreads * kLaunchRegs, "the shares must fit into the registers at launch");
+  static_assert(kN != 64 || kTileM * kN * 4 <= kStages * kStageBytes, "partial sums take the place of the stages");
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 };
 
 struct ProductArgs {
@@ -163,26 +255,62 @@ struct ProductArgs {
   void* c;
   const float* addend;  // fp32, C's layout, or null
   long long ldc;
-  int M, N, groups, tiles_m, tiles;
+  int M, N, groups, tiles_m, tiles, splits;
+  bool staged;  // results leave by TMA
   int* status;
 };
 
-template <int kN, bool kColumnScale, typename Out>
+// Four neighbouring results of one row, from a column that is a multiple of four.
+template <typename Out>
+__device__ __forceinline__ void store_quad(const ProductArgs& p, int row, int col, float4 v) {
+  if (row >= p.M || col >= p.N) return;
+  const long long at = row * p.ldc + col;
+  float x[4] = {v.x, v.y, v.z, v.w};
+  if (p.addend != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < p.N) x[k] += p.addend[at + k];
+  }
+  Out* dst = static_cast<Out*>(p.c) + at;
+  if ((p.ldc & 3) == 0) {  // whole quads, 16 or 8 bytes apart
+    if constexpr (sizeof(Out) == 4) {
+      *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      uint2 u;
+      *reinterpret_cast<__nv_bfloat162*>(&u.x) = __floats2bfloat162_rn(x[0], x[1]);
+      *reinterpret_cast<__nv_bfloat162*>(&u.y) = __floats2bfloat162_rn(x[2], x[3]);
+      *reinterpret_cast<uint2*>(dst) = u;
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (col + k >= p.N) continue;
+    if constexpr (sizeof(Out) == 4) dst[k] = x[k];
+    else dst[k] = __float2bfloat16_rn(x[k]);
+  }
+}
+
+template <int kN, bool kPair, bool kColumnScale, typename Out>
 __global__ void __launch_bounds__(kProductThreads, 1)
-fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs p) {
-  using C = ProductCfg<kN>;
+fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
+                  const __grid_constant__ ProductArgs p) {
+  using C = ProductCfg<kN, kPair, kColumnScale, Out>;
   constexpr int kStages = C::kStages, kBuffers = C::kBuffers, kOwn = C::kOwn;
-  constexpr uint32_t kIdesc = make_idesc(/*e4m3*/ 0, kTileM, kN);
+  constexpr uint32_t kIdesc = make_idesc(/*e4m3*/ 0, kPair ? 2 * kTileM : kTileM, kN);
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  float* col_scales = reinterpret_cast<float*>(smem + kStages * C::kStageBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(col_scales + C::kScaleFloats);
+  uint8_t* staging = smem + kStages * C::kStageBytes;
+  float* scales = reinterpret_cast<float*>(staging + C::kStagingBytes);  // [slot][kScaleFloats]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::kScaleSlots * C::kScaleFloats);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + kBuffers;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + kBuffers);
+  uint64_t* scale_full = acc_empty + kBuffers;
+  uint64_t* scale_empty = scale_full + C::kScaleSlots;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(scale_empty + C::kScaleSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert(2 * (kStages + kBuffers) * 8 + 8 <= C::kBarrierBytes, "barrier region");
+  static_assert(2 * (kStages + kBuffers + C::kScaleSlots) * 8 + 8 <= C::kBarrierBytes, "barrier region");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -192,152 +320,385 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
     for (int b = 0; b < kBuffers; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpilogueWarps);
+      mbar_init(&acc_empty[b], kPair ? 2 * kEpilogueWarps : kEpilogueWarps);
+    }
+    for (int i = 0; i < C::kScaleSlots; ++i) {
+      mbar_init(&scale_full[i], 32);
+      mbar_init(&scale_empty[i], kEpilogueWarps);
     }
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (warp == kEpilogueWarps + 1) {
-    tmem_alloc(tmem_holder, kN * kBuffers);
-    tmem_relinquish();
+  if (warp == 1) {
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_holder, kN * kBuffers);
+    } else {
+      tmem_alloc(tmem_holder, kN * kBuffers);
+      tmem_relinquish();
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) cg::this_cluster().sync();  // the other CTA's barriers exist
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_holder;
+  const int member = kPair ? static_cast<int>(blockIdx.x) & 1 : 0;  // of the pair
 
+  const int rank = kPair || p.splits == 1 ? 0 : static_cast<int>(blockIdx.x) % p.splits;
+  const int per_tile = kPair ? 2 : p.splits;  // CTAs
+  const int first_tile = static_cast<int>(blockIdx.x) / per_tile, tile_step = static_cast<int>(gridDim.x) / per_tile;
+  const int g0 = static_cast<int>(static_cast<long long>(p.groups) * rank / p.splits);
+  const int g1 = static_cast<int>(static_cast<long long>(p.groups) * (rank + 1) / p.splits);
   // Neighbouring tiles share operands: eight rows of tiles at a time, down the rows first.
   const int tiles_n = p.tiles / p.tiles_m;
   auto place = [&](int t, int& m0, int& n0) {
     const int band = t / (8 * tiles_n), in = t - band * 8 * tiles_n;
     const int high = min(8, p.tiles_m - band * 8);
-    m0 = (band * 8 + in % high) * kTileM;
+    m0 = (band * 8 + in % high) * (kPair ? 2 * kTileM : kTileM) + member * kTileM;
     n0 = in / high * kN;
   };
 
-  if (warp == kEpilogueWarps) {
-    if (lane == 0) {
+  if (warp < kFirstEpilogueWarp) {
+    if constexpr (C::kUneven) setmaxnreg_dec<C::kOtherRegs>();
+    // The whole warp walks the loops and one lane gives the commands: values that all lanes share stay in uniform registers, where
+    // the commands need them.  (With the loops inside one lane's branch the MMAs of a group took 660 clocks to issue, more than to run.)
+    if (warp == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
         int m0, n0;
         place(t, m0, n0);
-        for (int g = 0; g < p.groups; ++g) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
-            ok = false;
-            break;
+        for (int g = g0; g < g1; ++g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag));
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* s = smem + stage * C::kStageBytes;
+            if constexpr (kPair) {  // both CTAs' loads are counted by the barrier of the first
+              if (member == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::kStageBytes);
+              const uint32_t bar = cluster_addr(&full[stage], 0);
+              tma_load_2d_pair(s, &map_a, bar, g * kFp8Group, m0);
+              tma_load_2d_pair(s + kTileM * kFp8Group, &map_b, bar, g * kFp8Group, n0 + member * C::kRowsB);
+            } else {
+              mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+              tma_load_2d(s, &map_a, &full[stage], g * kFp8Group, m0);
+              tma_load_2d(s + kTileM * kFp8Group, &map_b, &full[stage], g * kFp8Group, n0);
+            }
           }
-          uint8_t* s = smem + stage * C::kStageBytes;
-          mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
-          tma_load_2d(s, &map_a, &full[stage], g * kFp8Group, m0);
-          tma_load_2d(s + kTileM * kFp8Group, &map_b, &full[stage], g * kFp8Group, n0);
+          __syncwarp();
           if (++stage == kStages) {
             stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    } else if (warp <= 2 && member == 0) {
+      // Two warps take the groups in turn: one waits for its operands and its buffer while the MMAs of the other run.  (A warp that has
+      // given commands is held until they start, so that with one warp its waits for the next group, some 300 clocks, lay between
+      // the MMAs: the products of 16384 x 2048 x 8192 took 3 us longer.)
+      static_assert(kStages % 2 == 0 && kBuffers % 2 == 0, "each warp has its own stages and buffers");
+      const long long mine = first_tile < p.tiles ? static_cast<long long>((p.tiles - 1 - first_tile) / tile_step + 1) * (g1 - g0) : 0;
+      int stage = warp - 1, buf = warp - 1;
+      uint32_t phase = 0, round = 0;
+      const uint64_t first_a = make_kmajor_sw128_desc(smem_u32(smem)), first_b = make_kmajor_sw128_desc(smem_u32(smem) + kTileM * kFp8Group);
+      for (long long i = warp - 1; i < mine; i += 2) {
+        const bool ok = mbar_wait(&full[stage], phase, abort_flag) && mbar_wait(&acc_empty[buf], round ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t a = first_a + stage * (C::kStageBytes >> 4), b = first_b + stage * (C::kStageBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < kFp8Group / 32; ++k) {
+            if constexpr (kPair) umma_f8_pair(tmem + buf * kN, a + 2 * k, b + 2 * k, kIdesc, k != 0);
+            else umma_f8(tmem + buf * kN, a + 2 * k, b + 2 * k, kIdesc, k != 0);
+          }
+          if constexpr (kPair) {
+            umma_commit_pair(&empty[stage]);
+            umma_commit_pair(&acc_full[buf]);
+          } else {
+            umma_commit(&empty[stage]);
+            umma_commit(&acc_full[buf]);
+          }
+        }
+        __syncwarp();
+        if ((stage += 2) >= kStages) {
+          stage -= kStages;
+          phase ^= 1;
+        }
+        if ((buf += 2) >= kBuffers) {
+          buf -= kBuffers;
+          round ^= 1;
+        }
+      }
+    } else if (warp == 3) {
+      // Scales: the epilogue would wait for the latency of their loads, some 800 clocks, once per group.
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
+        int m0, n0;
+        place(t, m0, n0);
+        for (int g = g0; g < g1; ++g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&scale_empty[slot], phase ^ 1, abort_flag));
+          if (!ok) break;
+          float* s = scales + slot * C::kScaleFloats;
+#pragma unroll
+          for (int i = lane; i < kTileM; i += 32) cp_async4(s + i, p.sa + min(m0 + i, p.M - 1) * p.sa_row + g * p.sa_group);
+          if constexpr (kColumnScale) {
+#pragma unroll
+            for (int i = lane; i < kN; i += 32) cp_async4(s + kTileM + i, p.sb + min(n0 + i, p.N - 1) * p.sb_row + g * p.sb_group);
+          } else if (lane < 2) {  // of the two halves of the tile's columns
+            cp_async4(s + kTileM + lane, p.sb + min(n0 + lane * kOwn, p.N - 1) / kFp8Group * p.sb_row + g * p.sb_group);
+          }
+          cp_async_arrive(&scale_full[slot]);
+          if (++slot == C::kScaleSlots) {
+            slot = 0;
             phase ^= 1;
           }
         }
       }
     }
-  } else if (warp == kEpilogueWarps + 1) {
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, round = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
-        for (int g = 0; g < p.groups; ++g) {
-          if (!mbar_wait(&acc_empty[buf], round ^ 1, abort_flag) || !mbar_wait(&full[stage], phase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
-          const uint32_t s = smem_u32(smem + stage * C::kStageBytes);
-          const uint64_t a = make_kmajor_sw128_desc(s), b = make_kmajor_sw128_desc(s + kTileM * kFp8Group);
-#pragma unroll
-          for (int k = 0; k < kFp8Group / 32; ++k) umma_f8(tmem + buf * kN, a + 2 * k, b + 2 * k, kIdesc, k != 0);
-          umma_commit(&empty[stage]);
-          umma_commit(&acc_full[buf]);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (++buf == kBuffers) {
-            buf = 0;
-            round ^= 1;
-          }
-        }
-      }
+    __syncwarp();
+    if (!kPair && p.splits > 1) {
+      cg::this_cluster().sync();
+      cg::this_cluster().sync();
     }
   } else {
-    const int stripe = warp & 3, half = warp >> 2;
-    float* my_scales = col_scales + warp * kOwn;
+    if constexpr (C::kUneven) setmaxnreg_inc<C::kEpilogueRegs>();
+    constexpr int kRowsOwn = kColumnScale ? 4 : 1;  // rows of a thread
+    const int stripe = warp & 3, half = (warp - kFirstEpilogueWarp) >> 2;
+    const int q = lane & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(stripe * 32) << 16) + half * kOwn;
-    int buf = 0;
-    uint32_t round = 0;
+    uint8_t* my_staging = staging + (warp - kFirstEpilogueWarp) * 32 * kOwn * 2;
+    const uint32_t own_rank = kPair ? member : rank;  // in the cluster
+    const uint32_t back_to_mma = cluster_addr(acc_empty, kPair ? 0 : own_rank), back_to_loads = cluster_addr(scale_empty, own_rank);
+    int buf = 0, slot = 0;
+    uint32_t round = 0, turn = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x) {
-      int m0, n0;
-      place(t, m0, n0);
-      const int row = m0 + stripe * 32 + lane, col0 = n0 + half * kOwn;
-      const float* sa = p.sa + min(row, p.M - 1) * p.sa_row;
-      float acc[kOwn];
+    for (int t = first_tile; t < p.tiles; t += tile_step) {
+      int row0, col0;
+      place(t, row0, col0);
+      const int row_in = stripe * 32 + (kColumnScale ? lane >> 2 : lane);  // of the tile: rows row_in + 8 i
+      row0 += row_in;
+      col0 += half * kOwn;
+      // Sums, in pairs.  Whole rows: two neighbouring columns.  Else sums[h * kOwn / 4 + i] for the rows row0 + 16 h and row0 + 16 h + 8 and the
+      // column 4 i + q.
+      uint64_t sums[kOwn / 2];
 #pragma unroll
-      for (int j = 0; j < kOwn; ++j) acc[j] = 0.f;
-      for (int g = 0; g < p.groups && ok; ++g) {
-        float scale = sa[g * p.sa_group];
-        if constexpr (kColumnScale) {
-          __syncwarp();
+      for (int i = 0; i < kOwn / 2; ++i) sums[i] = 0;
+      // Of the group that is being added: its scales and, in v, pieces of its sums.  The first piece of the next group is already on its way
+      // when the last one of this group is added.  (A wait that gave up lets everything run through; the flag is looked at below.)
+      constexpr int kPiece = kColumnScale || kN == 256 ? 32 : 16;                // columns
+      constexpr int kPieces = kColumnScale ? 2 * kOwn / kPiece : kOwn / kPiece;  // upper and lower 16 rows apart where B has a scale per row
+      constexpr int kQuarter = kPiece / 4;
+      uint32_t v[2][kColumnScale ? kPiece / 2 : kPiece];
+      float scale[kRowsOwn], s[kColumnScale ? kQuarter : 1];
+      const float* of_columns = nullptr;
+      auto issue = [&](int c) {
+        const uint32_t from = lanes + buf * kN;
+        if constexpr (kColumnScale) tmem_ld_16_issue(from + (static_cast<uint32_t>((c & 1) * 16) << 16) + (c >> 1) * kPiece, v[c & 1]);
+        else tmem_ld_32_issue(from + c * kPiece, v[c & 1]);
+      };
+      float next[kRowsOwn];
+      bool scales_there = false, sums_there = false;  // of the next group, as seen while this one is added
+      auto begin = [&]() {                            // of a group
+        if (!scales_there) mbar_wait(&scale_full[slot], turn, abort_flag);
+        const float* of_rows = scales + slot * C::kScaleFloats;
 #pragma unroll
-          for (int j = lane; j < kOwn; j += 32) my_scales[j] = p.sb[min(col0 + j, p.N - 1) * p.sb_row + g * p.sb_group];
-          __syncwarp();
-        } else {
-          scale *= p.sb[min(col0, p.N - 1) / kFp8Group * p.sb_row + g * p.sb_group];
-        }
-        ok = mbar_wait(&acc_full[buf], round, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        for (int i = 0; i < kRowsOwn; ++i) next[i] = of_rows[row_in + 8 * i];
+        if constexpr (!kColumnScale) next[0] *= of_rows[kTileM + half];
+        of_columns = of_rows + kTileM + half * kOwn;
+        if (!sums_there) mbar_wait(&acc_full[buf], round, abort_flag);
         tc_fence_after_sync();
-#pragma unroll
-        for (int c = 0; c < kOwn / 32; ++c) {
-          float v[32];
-          tmem_ld_32x32(lanes + buf * kN + c * 32, v);
-          if (c == kOwn / 32 - 1) {  // the buffer goes back to the MMAs
-            tc_fence_before_sync();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(kColumnScale ? v[j] * my_scales[c * 32 + j] : v[j], scale, acc[c * 32 + j]);
-        }
+        issue(0);
+      };
+      auto look = [&](bool at_sums) {
+        const bool last_buf = buf + 1 == kBuffers, last_slot = slot + 1 == C::kScaleSlots;
+        if (at_sums) sums_there = mbar_test(&acc_full[last_buf ? 0 : buf + 1], last_buf ? round ^ 1 : round);
+        else scales_there = mbar_test(&scale_full[last_slot ? 0 : slot + 1], last_slot ? turn ^ 1 : turn);
+      };
+      auto finish = [&]() {  // the buffer goes back to the MMAs, the scales' slot to their loads
+        tc_fence_before_sync();
+        mbar_arrive_at(back_to_mma + buf * 8, lane == 0);
+        mbar_arrive_at(back_to_loads + slot * 8, lane == 0);
         if (++buf == kBuffers) {
           buf = 0;
           round ^= 1;
         }
-      }
-      if (row >= p.M) continue;
-      Out* dst = static_cast<Out*>(p.c) + row * p.ldc;
-      const float* add = p.addend == nullptr ? nullptr : p.addend + row * p.ldc;
-      const bool vec = (p.ldc & 7) == 0;
-#pragma unroll
-      for (int j = 0; j < kOwn; j += 8) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          v[k] = ok ? acc[j + k] : __int_as_float(0x7fffffff);  // a pipeline that gave up leaves no plausible numbers
-          if (add != nullptr && col0 + j + k < p.N) v[k] += add[col0 + j + k];
+        if (++slot == C::kScaleSlots) {
+          slot = 0;
+          turn ^= 1;
         }
-        if (vec && col0 + j + 8 <= p.N) store8<true>(dst, col0 + j, p.N, v);
-        else store8<false>(dst, col0 + j, p.N, v);
+      };
+      if (g0 < g1) begin();
+      for (int g = g0; g < g1; ++g) {
+#pragma unroll
+        for (int i = 0; i < kRowsOwn; ++i) scale[i] = next[i];
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          if constexpr (kColumnScale) {
+            if ((c & 1) == 0) {
+#pragma unroll
+              for (int i = 0; i < kQuarter; ++i) s[i] = of_columns[(c >> 1) * kPiece + 4 * i + q];
+            }
+          }
+          uint64_t by = kColumnScale ? pack2(scale[kColumnScale ? 2 * (c & 1) : 0], scale[kColumnScale ? 2 * (c & 1) + 1 : 0]) : pack2(scale[0], scale[0]);
+          tmem_ld_wait(by);
+          if (c + 1 < kPieces) {
+            issue(c + 1);
+            if (c == 0) look(false);
+            if (c + 2 == kPieces) look(true);
+          } else {
+            finish();
+            if (kPieces > 1 && g + 1 < g1) begin();
+          }
+          if constexpr (!kColumnScale) {
+#pragma unroll
+            for (int j = 0; j < kPiece / 2; ++j) {
+              uint64_t& sum = sums[c * kPiece / 2 + j];
+              sum = fma2(pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), by, sum);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kQuarter; ++i) {
+              uint64_t& sum = sums[(c & 1) * (kOwn / 4) + (c >> 1) * kQuarter + i];
+              sum = fma2(mul2(pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), by), pack2(s[i], s[i]), sum);
+            }
+          }
+        }
+        if (kPieces == 1 && g + 1 < g1) begin();
+      }
+      ok = *abort_flag == 0;
+      float acc[kOwn];  // the same, row by row: [column] or [row0 + 8 i][column of this lane]
+#pragma unroll
+      for (int j = 0; j < kOwn / 2; ++j) {
+        float2 x = unpack2(sums[j]);
+        if (!ok) x = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));  // a pipeline that gave up leaves no plausible numbers
+        const int at = kColumnScale ? j / (kOwn / 4) * (kOwn / 2) + j % (kOwn / 4) : 2 * j;
+        acc[at] = x.x;
+        acc[at + (kColumnScale ? kOwn / 4 : 1)] = x.y;
+      }
+      if constexpr (kColumnScale) {
+        // Four lanes have every fourth column of a row: each takes four neighbours of sixteen.
+#pragma unroll
+        for (int i = 0; i < kOwn; i += 4) {
+          float* w = acc + i;
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const float got = __shfl_xor_sync(0xffffffffu, (q & 1) ? w[k] : w[k + 1], 1);
+            if (q & 1) w[k] = got;
+            else w[k + 1] = got;
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float got = __shfl_xor_sync(0xffffffffu, (q & 2) ? w[k] : w[k + 2], 2);
+            if (q & 2) w[k] = got;
+            else w[k + 2] = got;
+          }
+        }
+      }
+      // Quad j: four neighbouring columns of a row.
+      auto place_quad = [&](int j, int& row, int& col) {
+        row = kColumnScale ? row0 + 8 * (j / (kOwn / 16)) : row0;
+        col = kColumnScale ? col0 + 16 * (j % (kOwn / 16)) + 4 * q : col0 + 4 * j;
+      };
+      if (!kPair && p.splits > 1) {
+        // The stages are idle: every load has arrived and every MMA is done.  [quad][thread]
+        float4* mine = reinterpret_cast<float4*>(smem);
+        const int thread = threadIdx.x - 32 * kFirstEpilogueWarp;
+#pragma unroll
+        for (int j = 0; j < kOwn / 4; ++j) mine[j * 32 * kEpilogueWarps + thread] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        for (int j = kOwn / 4 * rank / p.splits; j < kOwn / 4 * (rank + 1) / p.splits; ++j) {
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int r = 0; r < p.splits; ++r) {
+            const float4 u = cluster.map_shared_rank(mine, r)[j * 32 * kEpilogueWarps + thread];
+            sum.x += u.x; sum.y += u.y; sum.z += u.z; sum.w += u.w;
+          }
+          int row, col;
+          place_quad(j, row, col);
+          store_quad<Out>(p, row, col, sum);
+        }
+        __syncwarp();
+        cluster.sync();  // nobody leaves while its sums are read
+        continue;
+      }
+      if (C::kStaged && p.staged) {
+        // 32 rows x 64 columns are 128 bytes a row, swizzled as TMA reads them: conflict-free, and the store itself runs beside the next tile.
+        if (lane == 0) bulk_wait_read();  // of the tile before
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kOwn / 64; ++c) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c * 64 + j * 8 + 2 * k], acc[c * 64 + j * 8 + 2 * k + 1]);
+              u[k] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            *reinterpret_cast<uint4*>(my_staging + c * 4096 + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          for (int c = 0; c < kOwn / 64; ++c)
+            if (row0 < p.M && col0 + c * 64 < p.N) tma_store_2d(&map_c, my_staging + c * 4096, col0 + c * 64, row0);
+          bulk_commit();
+        }
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < kOwn / 4; ++j) {
+        int row, col;
+        place_quad(j, row, col);
+        store_quad<Out>(p, row, col, make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]));
       }
     }
+    if (C::kStaged && lane == 0) bulk_wait_read();
     if (!ok && lane == 0) *p.status = 1;
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == kEpilogueWarps + 1) {
+  if constexpr (kPair) cg::this_cluster().sync();  // nothing of this CTA is read or signalled any more
+  if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, kN * kBuffers);
+    if constexpr (kPair) tmem_dealloc_pair(tmem, kN * kBuffers);
+    else tmem_dealloc(tmem, kN * kBuffers);
   }
+  if constexpr (kPair) cg::this_cluster().sync();
+}
+
+// Once per kernel and device: room in shared memory, and that a kernel which moves registers between its warpgroups
+// has the registers at launch that it was written for (an increase beyond them would wait forever).
+void prepare_product(const void* kernel, int smem, int launch_regs) {
+  static std::mutex mutex;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mutex);
+  if (!done.insert({kernel, device}).second) return;
+  if (launch_regs > 0) {
+    cudaFuncAttributes attr;
+    C10_CUDA_CHECK(cudaFuncGetAttributes(&attr, kernel));
+    TORCH_CHECK(attr.numRegs >= launch_regs, "fp8: the product was built with ", attr.numRegs, " registers per thread; it needs ", launch_regs);
+  }
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+}
+
+// Results [M, N] in bf16, in boxes of 32 rows and 64 columns.
+CUtensorMap result_map(const torch::Tensor& out, int64_t M, int64_t N) {
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(N) * 2};
+  const cuuint32_t box[2] = {64, 32}, elem_strides[2] = {1, 1};
+  const CUresult res = get_encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out.data_ptr(), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(res));
+  return map;
 }
 
 CUtensorMap operand_map(const torch::Tensor& t, int box_rows) {
@@ -401,7 +762,7 @@ std::tuple<torch::Tensor, torch::Tensor> fp8_rows(const torch::Tensor& x) {
   auto q = bytes_of(x, T, K);
   auto scale = torch::empty({G, T}, x.options().dtype(torch::kFloat32));
   if (T == 0 || K == 0) return {q, scale};
-  const int64_t grid = (T * G * 16 + kRowsThreads - 1) / kRowsThreads;
+  const int64_t sets = (T * G + kRowsAtOnce - 1) / kRowsAtOnce, grid = (sets * 16 + kRowsThreads - 1) / kRowsThreads;
   TORCH_CHECK(grid < (1LL << 31), "fp8: the source is too large");
   auto st = at::cuda::getCurrentCUDAStream();
   with_source(x, [&](auto* p, auto vec) {
@@ -455,9 +816,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fp8_squares(const torch:
 }
 
 // a [M, K], b [N, K] e4m3 bytes; sa [M, groups]; sb [N, groups] or, per block of 128 rows of b, [ceil(N / 128), groups]; any strides.
-// -> a b' [M, N] in fp32 or bf16, plus `addend` (fp32 [M, N]).
+// -> a b' [M, N] in fp32 or bf16, plus `addend` (fp32 [M, N]); as a tensor of `shape` where that is given.
 torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb, bool column_scales, bool out_bf16,
-                         const std::optional<torch::Tensor>& addend, torch::Tensor status) {
+                         const std::optional<torch::Tensor>& addend, torch::Tensor status, std::optional<std::vector<int64_t>> shape) {
   check_operand(a, sa, "a");
   check_operand(b, sb, "b");
   const int64_t M = a.size(0), N = b.size(0), K = a.size(1);
@@ -465,7 +826,8 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
   TORCH_CHECK(sa.size(0) == M && sb.size(0) == (column_scales ? N : groups_of(N)), "fp8: rows of the scales");
   TORCH_CHECK(status.device() == a.device() && status.scalar_type() == torch::kInt32 && status.numel() == 1, "fp8: status is one int32");
   c10::cuda::CUDAGuard guard(a.device());
-  auto out = torch::empty({M, N}, sa.options().dtype(out_bf16 ? torch::kBFloat16 : torch::kFloat32));
+  auto out = torch::empty(shape.has_value() ? *shape : std::vector<int64_t>{M, N}, sa.options().dtype(out_bf16 ? torch::kBFloat16 : torch::kFloat32));
+  TORCH_CHECK(out.numel() == M * N, "fp8: shape of the result");
   if (addend.has_value())
     TORCH_CHECK(addend->device() == a.device() && addend->scalar_type() == torch::kFloat32 && addend->is_contiguous() && addend->sizes() == out.sizes(), "fp8: the addend is fp32 [M, N]");
   if (out.numel() == 0) return out;
@@ -474,22 +836,57 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
   auto st = at::cuda::getCurrentCUDAStream();
   ProductArgs p{sa.data_ptr<float>(), sb.data_ptr<float>(), sa.stride(0), sa.stride(1), sb.stride(0), sb.stride(1), out.data_ptr(),
                 addend.has_value() ? addend->data_ptr<float>() : nullptr, N, static_cast<int>(M), static_cast<int>(N), static_cast<int>(groups_of(K)),
-                static_cast<int>((M + kTileM - 1) / kTileM), 0, status.data_ptr<int>()};
-  auto go = [&](auto n, auto column, auto out_tag) {
+                static_cast<int>((M + kTileM - 1) / kTileM), 0, 1, out_bf16 && !addend.has_value() && N % 8 == 0, status.data_ptr<int>()};
+  auto go = [&](auto n, auto pair, auto column, auto out_tag, int splits) {
     constexpr int kN = decltype(n)::value;
+    constexpr bool kPair = decltype(pair)::value;
     using Out = decltype(out_tag);
-    using Cfg = ProductCfg<kN>;
+    using Cfg = ProductCfg<kN, kPair, decltype(column)::value, Out>;
+    constexpr int kRows = kPair ? 2 * kTileM : kTileM;
+    p.tiles_m = static_cast<int>((M + kRows - 1) / kRows);
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((N + kN - 1) / kN);
     TORCH_CHECK(tiles < (1LL << 31), "fp8: the product is too large");
     p.tiles = static_cast<int>(tiles);
-    auto* kernel = fp8_matmul_kernel<kN, decltype(column)::value, Out>;
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
-    kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, sms)), kProductThreads, Cfg::kSmemBytes, st>>>(operand_map(a, kTileM), operand_map(b, kN), p);
+    p.splits = splits;
+    const CUtensorMap map_a = operand_map(a, kTileM), map_b = operand_map(b, Cfg::kRowsB);
+    const CUtensorMap map_c = Cfg::kStaged && p.staged ? result_map(out, M, N) : map_a;
+    auto* kernel = fp8_matmul_kernel<kN, kPair, decltype(column)::value, Out>;
+    prepare_product(reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes, Cfg::kUneven ? Cfg::kLaunchRegs : 0);
+    cudaLaunchConfig_t cfg{};
+    const int per_tile = kPair ? 2 : p.splits;  // CTAs, one cluster
+    cfg.gridDim = dim3(p.splits > 1 ? p.tiles * p.splits : static_cast<unsigned>(std::min<int64_t>(tiles, sms / per_tile)) * per_tile);
+    cfg.blockDim = dim3(kProductThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(per_tile), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = per_tile > 1 ? 1 : 0;
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_c, p));
   };
+  // The shape of a tile by what the product would take with it: waves of tiles times the time of one group step of a tile, in units of a step of 128 x 128
+  // (measured on 16384 x 8192 x 2048: 269 us with pairs, 326 with 128 x 128, 644 with 128 x 64; a scale per row of B: 482, 499 as pairs of 256 x 128,
+  // 695).  Narrow tiles are cut along K among up to eight CTAs while SMs are idle; joining them takes about two steps.
   auto with_n = [&](auto column, auto out_tag) {
-    if (p.tiles_m * ((N + 255) / 256) >= sms) go(std::integral_constant<int, 256>{}, column, out_tag);
-    else if (p.tiles_m * ((N + 127) / 128) >= sms) go(std::integral_constant<int, 128>{}, column, out_tag);
-    else go(std::integral_constant<int, 64>{}, column, out_tag);
+    constexpr bool kColumn = decltype(column)::value;
+    auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    const double wide_step = kColumn ? 1.93 : 1.63, narrow_step = kColumn ? 0.7 : 1.0;
+    const double wide = up(up(M, 256) * up(N, 256), sms / 2) * wide_step * p.groups;
+    const double middle = (kColumn ? up(up(M, 256) * up(N, 128), sms / 2) : up(up(M, 128) * up(N, 128), sms)) * static_cast<double>(p.groups);
+    const int64_t narrow_tiles = up(M, 128) * up(N, 64);
+    double narrow = 1e300;
+    int splits = 1;
+    for (int s = 1; s <= kMaxSplits && (s == 1 || (narrow_tiles * s <= sms && p.groups >= 2 * s)); s *= 2) {
+      const double t = up(narrow_tiles * s, sms) * narrow_step * up(p.groups, s) + (s > 1 ? 2. : 0.);
+      if (t < narrow) {
+        narrow = t;
+        splits = s;
+      }
+    }
+    if (wide <= middle && wide <= narrow) go(std::integral_constant<int, 256>{}, std::true_type{}, column, out_tag, 1);
+    else if (middle <= narrow) go(std::integral_constant<int, 128>{}, std::integral_constant<bool, kColumn>{}, column, out_tag, 1);
+    else go(std::integral_constant<int, 64>{}, std::false_type{}, column, out_tag, splits);
   };
   auto with_out = [&](auto column) {
     if (out_bf16) with_n(column, bf16{});
@@ -505,7 +902,9 @@ void register_fp8_ops(pybind11::module_& m) {
   m.def("fp8_rows", &fp8_rows);
   m.def("fp8_both", &fp8_both);
   m.def("fp8_squares", &fp8_squares);
-  m.def("fp8_matmul", &fp8_matmul);
+  namespace py = pybind11;
+  m.def("fp8_matmul", &fp8_matmul, py::arg("a"), py::arg("sa"), py::arg("b"), py::arg("sb"), py::arg("column_scales"), py::arg("out_bf16"), py::arg("addend"),
+        py::arg("status"), py::arg("shape") = py::none());
 }
 
 }  // namespace ob200

@@ -36,9 +36,10 @@ __device__ __forceinline__ float row_sum(float v, float* parts, int warps_per_ro
   return s;
 }
 
+template <bool kVec>
 __device__ __forceinline__ void load_weight(const void* w, bool w_bf16, int col, int C, float (&v)[8]) {
-  if (w_bf16) load8<false>(static_cast<const bf16*>(w), col, C, v);
-  else load8<false>(static_cast<const float*>(w), col, C, v);
+  if (w_bf16) load8<kVec>(static_cast<const bf16*>(w), col, C, v);
+  else load8<kVec>(static_cast<const float*>(w), col, C, v);
 }
 
 struct NormFwdArgs {
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) add_norm_fwd_kernel(const NormFwdArg
   for (int v = 0; v < kVecs; ++v) {
     const int col = (v * a.tpr + t) * 8;
     float w[8];
-    load_weight(a.w, a.w_bf16, col, C, w);
+    load_weight<kVec>(a.w, a.w_bf16, col, C, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) h[v][k] = h[v][k] * rs * w[k];
     if (a.out == kOutFp8) {
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) add_norm_bwd_kernel(const NormBwdArg
       load8<kVec>(static_cast<const R*>(a.h) + at, col, C, z[v]);
       if (a.dy_bf16) load8<kVec>(static_cast<const bf16*>(a.dy) + at, col, C, g[v]);
       else load8<kVec>(static_cast<const float*>(a.dy) + at, col, C, g[v]);
-      load_weight(a.w, a.w_bf16, col, C, w);
+      load_weight<kVec>(a.w, a.w_bf16, col, C, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         z[v][k] *= rs;
@@ -217,14 +218,14 @@ bool is_bf16(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat1
 bool fp32_or_bf16(const torch::Tensor& t) { return t.scalar_type() == torch::kFloat32 || is_bf16(t); }
 
 void check_rows(const torch::Tensor& x, const char* what) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous() && fp32_or_bf16(x), "add_norm: ", what, " is a contiguous fp32 or bf16 CUDA matrix");
-  TORCH_CHECK(x.size(1) > 0 && x.size(1) <= kMaxNormWidth, "add_norm: rows have 1 to ", kMaxNormWidth, " columns");
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.is_contiguous() && fp32_or_bf16(x), "add_norm: ", what, " is a contiguous fp32 or bf16 CUDA tensor");
+  TORCH_CHECK(x.size(-1) > 0 && x.size(-1) <= kMaxNormWidth, "add_norm: rows have 1 to ", kMaxNormWidth, " columns");
 }
 void check_like(const torch::Tensor& t, const torch::Tensor& x, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.is_contiguous() && fp32_or_bf16(t) && t.sizes() == x.sizes(), "add_norm: ", what, " is fp32 or bf16, of x's shape");
 }
 void check_weight(const torch::Tensor& w, const torch::Tensor& x) {
-  TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.is_contiguous() && fp32_or_bf16(w) && w.numel() == x.size(1), "add_norm: the weight is fp32 or bf16 [C]");
+  TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.is_contiguous() && fp32_or_bf16(w) && w.numel() == x.size(-1), "add_norm: the weight is fp32 or bf16 [C]");
 }
 
 template <typename F>
@@ -252,7 +253,7 @@ void with_shape(const NormShape& s, bool vec, F&& f) {
 
 int64_t add_norm_max_width() { return kMaxNormWidth; }
 
-// x, r [rows, C] (r may be absent; fp32 x with bf16 r is not offered) -> (y, scale, h, rstd).  out: 0 fp32, 1 bf16, 2 e4m3 (uint8, rows at a
+// x, r [..., C] (r may be absent; fp32 x with bf16 r is not offered) -> (y, scale, h, rstd).  out: 0 fp32, 1 bf16, 2 e4m3 (uint8, rows at a
 // pitch of a multiple of 16 bytes) with scale [groups, rows].  h is empty where r is absent (it is x then).
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> add_norm_fwd(const torch::Tensor& x, const std::optional<torch::Tensor>& r,
                                                                                     const torch::Tensor& w, double eps, int64_t out, bool want_rstd) {
@@ -261,17 +262,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> add_norm_
   if (r.has_value()) check_like(*r, x, "the residual");
   TORCH_CHECK(!r.has_value() || is_bf16(x) || !is_bf16(*r), "add_norm: an fp32 x needs an fp32 residual");
   TORCH_CHECK(out >= 0 && out <= 2, "add_norm: output format");
-  const int64_t rows = x.size(0), C = x.size(1);
+  const int64_t C = x.size(-1), rows = x.numel() / C;
   c10::cuda::CUDAGuard guard(x.device());
   const auto opt = x.options();
   const int64_t pitch = (C + 15) / 16 * 16, groups = (C + kFp8Group - 1) / kFp8Group;
-  auto y = out == kOutFp8 ? torch::empty({rows, pitch}, opt.dtype(torch::kUInt8)) : torch::empty({rows, C}, opt.dtype(out == kOutBf16 ? torch::kBFloat16 : torch::kFloat32));
+  auto y = out == kOutFp8 ? torch::empty({rows, pitch}, opt.dtype(torch::kUInt8)) : torch::empty(x.sizes(), opt.dtype(out == kOutBf16 ? torch::kBFloat16 : torch::kFloat32));
   auto scale = torch::empty({out == kOutFp8 ? groups : 0, rows}, opt.dtype(torch::kFloat32));
   auto h = r.has_value() ? torch::empty_like(*r) : torch::empty({0}, opt);
   auto rstd = torch::empty({want_rstd ? rows : 0}, opt.dtype(torch::kFloat32));
   if (rows == 0) return {y, scale, h, rstd};
   const NormShape s = norm_shape(C);
-  const bool vec = C % 8 == 0 && aligned16(x.data_ptr()) && (!r.has_value() || aligned16(r->data_ptr()));
+  const bool vec = C % 8 == 0 && aligned16(w.data_ptr()) && aligned16(x.data_ptr()) && (!r.has_value() || aligned16(r->data_ptr()));
   const NormFwdArgs args{x.data_ptr(), r.has_value() ? r->data_ptr() : nullptr, w.data_ptr(), r.has_value() ? h.data_ptr() : nullptr, y.data_ptr(),
                          want_rstd ? rstd.data_ptr<float>() : nullptr, scale.data_ptr<float>(), rows, static_cast<int>(C), s.tpr, static_cast<int>(out),
                          static_cast<int>(pitch), is_bf16(w), static_cast<float>(eps)};
@@ -298,16 +299,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> add_norm_bwd(const torch
     check_like(*dh, h, "dh");
     TORCH_CHECK(dh->scalar_type() == h.scalar_type(), "add_norm: dh has h's type");
   }
-  const int64_t rows = h.size(0), C = h.size(1);
+  const int64_t C = h.size(-1), rows = h.numel() / C;
   TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == torch::kFloat32 && rstd.is_contiguous() && rstd.numel() == rows, "add_norm: rstd fp32 [rows]");
   TORCH_CHECK(dx_bf16 || !is_bf16(h), "add_norm: an fp32 x has an fp32 h");
   c10::cuda::CUDAGuard guard(h.device());
-  auto dx = torch::empty({rows, C}, h.options().dtype(dx_bf16 ? torch::kBFloat16 : torch::kFloat32));
+  auto dx = torch::empty(h.sizes(), h.options().dtype(dx_bf16 ? torch::kBFloat16 : torch::kFloat32));
   auto dr = want_dr ? torch::empty_like(h) : torch::empty({0}, h.options());
   auto dw = torch::empty({C}, w.options());
   if (rows == 0) return {dx, dr, dw.zero_()};
   const NormShape s = norm_shape(C);
-  const bool vec = C % 8 == 0 && aligned16(h.data_ptr()) && aligned16(dy.data_ptr()) && (!dh.has_value() || aligned16(dh->data_ptr()));
+  const bool vec = C % 8 == 0 && aligned16(w.data_ptr()) && aligned16(h.data_ptr()) && aligned16(dy.data_ptr()) && (!dh.has_value() || aligned16(dh->data_ptr()));
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   const int threads = s.tpr * s.per_cta;
   const int64_t sets = (rows + s.per_cta - 1) / s.per_cta;

@@ -279,14 +279,14 @@ def test_llama_runs_all_of_it_together():
 
     model, plain = _llama(fp8=True, fused_embedding=True), _llama()
     idx = torch.randint(0, 500, (3, 34), device="cuda")
-    count = fused_ops.launch_count
+    count = fused_ops.launches()
     losses = []
     for m in (model, plain):
         with torch.autocast("cuda", dtype=BF16):
             loss = m(idx[:, :-1], idx[:, 1:])
         loss.backward()
         losses.append(float(loss))
-    assert fused_ops.launch_count > count
+    assert fused_ops.launches() > count
     # two layers whose products are off by about 2^-5 rms each, in a loss of about log 500 over random weights of 0.02
     assert abs(losses[0] - losses[1]) < 0.05
     for (name, a), (_, b) in zip(model.named_parameters(), plain.named_parameters()):
