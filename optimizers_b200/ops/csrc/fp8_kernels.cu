@@ -245,7 +245,7 @@ struct ProductCfg {
   static constexpr bool kUneven = kN == 256;
   static constexpr int kLaunchRegs = 168, kEpilogueRegs = 232, kOtherRegs = 40;
   static_assert(256 * kEpilogueRegs + 128 * kOtherRegs <= kProductThreads * kLaunchRegs, "the shares must fit into the registers at launch");
-  static_assert(kN != 64 || kTileM * kN * 4 <= kStages * kStageBytes, "partial sums take the place of the stages");
+  static_assert(kN == 256 || kTileM * kN * 4 <= kStages * kStageBytes, "partial sums take the place of the stages");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -625,7 +625,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         cluster.sync();  // nobody leaves while its sums are read
         continue;
       }
-      if (C::kStaged && p.staged) {
+      if (C::kStaged && p.addend == nullptr) {
         // 32 rows x 64 columns are 128 bytes a row, swizzled as TMA reads them: conflict-free, and the store itself runs beside the next tile.
         if (lane == 0) bulk_wait_read();  // of the tile before
         __syncwarp();
@@ -641,6 +641,20 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             *reinterpret_cast<uint4*>(my_staging + c * 4096 + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
           }
+        }
+        if (!p.staged) {  // rows that TMA cannot write (their pitch is no multiple of 16 bytes): neighbouring lanes store neighbours
+          __syncwarp();
+          const int from = row0 - lane;
+          for (int r = 0; r < 32 && from + r < p.M; ++r) {
+            bf16* dst = static_cast<bf16*>(p.c) + (from + r) * p.ldc;
+#pragma unroll
+            for (int c = lane; c < kOwn; c += 32) {
+              const uint8_t* at = my_staging + (c / 64) * 4096 + r * 128 + ((((c % 64) / 8) ^ (r & 7)) << 4) + (c % 8) * 2;
+              if (col0 + c < p.N) dst[col0 + c] = *reinterpret_cast<const bf16*>(at);
+            }
+          }
+          __syncwarp();
+          continue;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -867,26 +881,30 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
   };
   // The shape of a tile by what the product would take with it: waves of tiles times the time of one group step of a tile, in units of a step of 128 x 128
   // (measured on 16384 x 8192 x 2048: 269 us with pairs, 326 with 128 x 128, 644 with 128 x 64; a scale per row of B: 482, 499 as pairs of 256 x 128,
-  // 695).  Narrow tiles are cut along K among up to eight CTAs while SMs are idle; joining them takes about two steps.
+  // 695).  Tiles of single CTAs are cut along K among up to eight while SMs are idle; joining them takes about two steps.
   auto with_n = [&](auto column, auto out_tag) {
     constexpr bool kColumn = decltype(column)::value;
     auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
     const double wide_step = kColumn ? 1.93 : 1.63, narrow_step = kColumn ? 0.7 : 1.0;
     const double wide = up(up(M, 256) * up(N, 256), sms / 2) * wide_step * p.groups;
     const double middle = (kColumn ? up(up(M, 256) * up(N, 128), sms / 2) : up(up(M, 128) * up(N, 128), sms)) * static_cast<double>(p.groups);
-    const int64_t narrow_tiles = up(M, 128) * up(N, 64);
-    double narrow = 1e300;
-    int splits = 1;
-    for (int s = 1; s <= kMaxSplits && (s == 1 || (narrow_tiles * s <= sms && p.groups >= 2 * s)); s *= 2) {
-      const double t = up(narrow_tiles * s, sms) * narrow_step * up(p.groups, s) + (s > 1 ? 2. : 0.);
-      if (t < narrow) {
-        narrow = t;
-        splits = s;
+    double best = std::min(wide, middle);
+    int cut_n = 0, splits = 1;
+    for (int n : {64, 128}) {
+      const int64_t tiles = up(M, 128) * up(N, n);
+      for (int s = n == 64 ? 1 : 2; s <= kMaxSplits && (s == 1 || (tiles * s <= sms && p.groups >= 2 * s)); s *= 2) {
+        const double t = up(tiles * s, sms) * (n == 64 ? narrow_step : 1.) * up(p.groups, s) + (s > 1 ? 2. : 0.);
+        if (t < best) {
+          best = t;
+          cut_n = n;
+          splits = s;
+        }
       }
     }
-    if (wide <= middle && wide <= narrow) go(std::integral_constant<int, 256>{}, std::true_type{}, column, out_tag, 1);
-    else if (middle <= narrow) go(std::integral_constant<int, 128>{}, std::integral_constant<bool, kColumn>{}, column, out_tag, 1);
-    else go(std::integral_constant<int, 64>{}, std::false_type{}, column, out_tag, splits);
+    if (cut_n == 64) go(std::integral_constant<int, 64>{}, std::false_type{}, column, out_tag, splits);
+    else if (cut_n == 128) go(std::integral_constant<int, 128>{}, std::false_type{}, column, out_tag, splits);
+    else if (wide <= middle) go(std::integral_constant<int, 256>{}, std::true_type{}, column, out_tag, 1);
+    else go(std::integral_constant<int, 128>{}, std::integral_constant<bool, kColumn>{}, column, out_tag, 1);
   };
   auto with_out = [&](auto column) {
     if (out_bf16) with_n(column, bf16{});
