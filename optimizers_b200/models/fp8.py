@@ -42,7 +42,7 @@ def _groups(n: int) -> int:
     return -(-n // GROUP)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Rows:
     """[T, K] e4m3 values and fp32 scales [T, ceil(K / 128)]."""
 
@@ -56,7 +56,7 @@ class Rows:
         return _values(self.data, self.scale, 1)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Weight:
     """[N, K] e4m3 values and fp32 scales [ceil(N / 128), ceil(K / 128)] of a linear layer's weight."""
 
@@ -96,6 +96,8 @@ def check_status() -> None:
 def _status_of(device: torch.device) -> Tensor:
     status = _status.get(device)
     if status is None:
+        if torch.cuda.is_current_stream_capturing():  # it would live in that graph's memory
+            raise RuntimeError("call fp8.linear once on this device before capturing it into a CUDA graph")
         status = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
     return status
 
@@ -129,30 +131,20 @@ def _rows(x: Tensor, native: bool) -> tuple[Tensor, Tensor]:
     return _e4m3(raw, x.shape[1]), scale.t()
 
 
-def _both(x: Tensor, native: bool) -> tuple[tuple[Tensor, Tensor], tuple[Tensor, Tensor]]:
-    """x and its transpose, each in groups along its own rows."""
+def _squares(w: Tensor, native: bool) -> tuple[Tensor, Tensor]:
     if not native:
-        return _plain_groups(x, 1), _plain_groups(x.t(), 1)
-    raw, scale, raw_t, scale_t = fused_ops._ext().fp8_both(_source(x))
+        return _plain_groups(w, GROUP)
+    raw, _, scale = fused_ops._ext().fp8_squares(_source(w), False)
     fused_ops._count()
-    return (_e4m3(raw, x.shape[1]), scale.t()), (_e4m3(raw_t, x.shape[0]), scale_t.t())
+    return _e4m3(raw, w.shape[1]), scale
 
 
-def _squares(w: Tensor, transpose: bool, native: bool) -> tuple[tuple[Tensor, Tensor], tuple[Tensor, Tensor] | None]:
+def _product(a, b, dtype: torch.dtype, native: bool, shape) -> Tensor:
+    """``a @ b.T`` in ``dtype`` as a tensor of ``shape``, for rows a and a weight's squares b."""
     if not native:
-        data, scale = _plain_groups(w, GROUP)
-        return (data, scale), (data.t(), scale.t())
-    raw, raw_t, scale = fused_ops._ext().fp8_squares(_source(w), transpose)
-    fused_ops._count()
-    return (_e4m3(raw, w.shape[1]), scale), (_e4m3(raw_t, w.shape[0]), scale.t()) if transpose else None
-
-
-def _product(a, b, column_scales: bool, dtype: torch.dtype, native: bool, addend: Tensor | None = None, shape=None) -> Tensor:
-    """``a @ b.T`` (+ addend, fp32) in ``dtype``; b has a scale per row (``column_scales``) or per 128 rows."""
-    if not native:
-        return _plain_product(a, b, 1 if column_scales else GROUP, dtype)
+        return _plain_product(a, b, GROUP, dtype).view(shape)
     out = fused_ops._ext().fp8_matmul(
-        a[0].view(torch.uint8), a[1], b[0].view(torch.uint8), b[1], column_scales, dtype == torch.bfloat16, addend, _status_of(a[0].device), shape
+        a[0].view(torch.uint8), a[1], b[0].view(torch.uint8), b[1], False, dtype == torch.bfloat16, None, _status_of(a[0].device), shape
     )
     fused_ops._count()
     return out
@@ -199,7 +191,7 @@ def quantize_weight(weight: Tensor) -> Weight:
     if weight.dim() != 2:
         raise ValueError(f"a weight is a matrix, got shape {tuple(weight.shape)}")
     w = weight.detach()
-    return Weight(*_squares(w, False, _is_native(w))[0])
+    return Weight(*_squares(w, _is_native(w)))
 
 
 @torch.no_grad()
@@ -270,11 +262,13 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
         raise ValueError("linear needs a weight")
     held_x = isinstance(x, Rows)
     source = x.data if held_x else x
+    if source.dim() < 1 or source.shape[-1] == 0:
+        raise ValueError(f"linear takes rows of at least one value, got shape {tuple(source.shape)}")
     tensors, empty = [], source.numel() == 0
     for w in weights:
         held = isinstance(w, Weight)
         data = w.data if held else w
-        if data.dim() != 2 or source.dim() < 1 or data.shape[1] != source.shape[-1]:
+        if data.dim() != 2 or data.shape[1] != source.shape[-1]:
             raise ValueError(f"a weight of shape {tuple(data.shape)} does not fit rows of shape {tuple(source.shape)}")
         if data.device != source.device:
             raise ValueError(f"weight on {data.device}, x on {source.device}")
@@ -287,14 +281,18 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
         raise ValueError("linear takes and returns floating-point tensors")
     operands = tensors if held_x else [x, *tensors]
     native = not empty and out_dtype in _SOURCES and (fused_ops._kernels_take(*operands) if operands else fused_ops._native(source))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
-        if held_x or len(tensors) < len(weights):
-            raise ValueError("operands held in 8 bits carry no gradient: pass tensors for x and every weight in training, or use torch.no_grad()")
-        if native:
-            out = fused_ops._ext().fp8_linear(x, tensors, out_dtype == torch.bfloat16, _status_of(x.device))
-        else:
-            out = _Linear.apply(x.reshape(-1, x.shape[-1]), out_dtype, *tensors)
-            out = [y.view(*x.shape[:-1], y.shape[-1]) for y in out]
+    learns = torch.is_grad_enabled() and any(t.requires_grad for t in operands)
+    if learns and (held_x or len(tensors) < len(weights)):
+        raise ValueError("operands held in 8 bits carry no gradient: pass tensors for x and every weight in training, or use torch.no_grad()")
+    if native and not held_x and len(tensors) == len(weights):
+        out = fused_ops._ext().fp8_linear(x, tensors, out_dtype == torch.bfloat16, _status_of(x.device))
+    elif native and not held_x and not tensors:
+        out = fused_ops._ext().fp8_linear_held(
+            x, [_aligned(w.data) for w in weights], [w.scale for w in weights], out_dtype == torch.bfloat16, _status_of(x.device)
+        )
+    elif learns:
+        out = _Linear.apply(x.reshape(-1, x.shape[-1]), out_dtype, *tensors)
+        out = [y.view(*x.shape[:-1], y.shape[-1]) for y in out]
     else:
         rows = (x.data, x.scale) if held_x else _rows(x.detach().reshape(-1, x.shape[-1]), native)
         if native and held_x:
@@ -304,7 +302,6 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
             if isinstance(w, Weight):
                 held = (_aligned(w.data) if native else w.data, w.scale)
             else:
-                held = _squares(w.detach(), False, native)[0]
-            shape = [*source.shape[:-1], held[0].shape[0]]
-            out.append(_product(rows, held, False, out_dtype, native, shape=shape) if native else _product(rows, held, False, out_dtype, False).view(shape))
+                held = _squares(w.detach(), native)
+            out.append(_product(rows, held, out_dtype, native, [*source.shape[:-1], held[0].shape[0]]))
     return tuple(out) if several else out[0]

@@ -198,7 +198,7 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
 # Residual addition + RMSNorm
 # --------------------------------------------------------------------------------------------------
 def _check_add_norm(x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
-    if x.dim() < 1 or weight.shape != x.shape[-1:]:
+    if x.dim() < 1 or x.shape[-1] == 0 or weight.shape != x.shape[-1:]:
         raise ValueError(f"a norm weight of shape {tuple(weight.shape)} does not fit rows of shape {tuple(x.shape)}")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"x and residual differ in shape: {tuple(x.shape)} and {tuple(residual.shape)}")
@@ -206,7 +206,7 @@ def _check_add_norm(x: Tensor, residual: Tensor | None, weight: Tensor) -> None:
         raise ValueError("add_rms_norm takes floating-point tensors")
 
 
-_MOST_COLUMNS = 16384  # of a row that the kernels take
+_MOST_COLUMNS = 16384  # of a row that the norm kernels take
 _KINDS = (torch.float32, torch.bfloat16)
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _on_sm100: dict[int | None, bool] = {}

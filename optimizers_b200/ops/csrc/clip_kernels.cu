@@ -304,6 +304,8 @@ torch::Tensor clip_scale(const std::vector<torch::Tensor>& grads, const torch::T
                                                      static_cast<float>(max_norm), batch == 0 ? norm.data_ptr<float>() : nullptr);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   });
+  for (const auto& g : grads)  // written in place: whoever saved one for a backward pass has to learn of it
+    if (!g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

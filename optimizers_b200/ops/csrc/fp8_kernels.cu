@@ -102,13 +102,84 @@ fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
   }
 }
 
+// Eight rows of eight neighbouring values as a thread of the tile kernel holds them.  bf16 stays packed: half the registers, and
+// magnitudes are compared two at a time as 16-bit integers.
+template <typename T>
+struct Patch {
+  float v[8][8];
+  template <bool kVec>
+  __device__ __forceinline__ void load(int r, const float* row, int col, int cols) { load8<kVec>(row, col, cols, v[r]); }
+  __device__ __forceinline__ void clear(int r) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[r][k] = 0.f;
+  }
+  __device__ __forceinline__ float at(int r, int k) const { return v[r][k]; }
+  __device__ __forceinline__ uint32_t row_top(int r) const { return top_of(v[r]); }
+  __device__ __forceinline__ void column_tops(uint32_t (&down)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) t = max(t, magnitude_bits(v[r][k]));
+      down[k] = max(t, __shfl_xor_sync(0xffffffffu, t, 16));
+    }
+  }
+};
+
+template <>
+struct Patch<bf16> {
+  uint32_t w[8][4];
+  template <bool kVec>
+  __device__ __forceinline__ void load(int r, const bf16* row, int col, int cols) {
+    if constexpr (kVec) {
+      const uint4 u = col < cols ? *reinterpret_cast<const uint4*>(row + col) : make_uint4(0u, 0u, 0u, 0u);
+      w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+    } else {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = col + 2 * k < cols ? h[col + 2 * k] : 0u, hi = col + 2 * k + 1 < cols ? h[col + 2 * k + 1] : 0u;
+        w[r][k] = lo | (hi << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void clear(int r) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[r][k] = 0;
+  }
+  __device__ __forceinline__ float at(int r, int k) const { return __uint_as_float((k & 1) ? w[r][k >> 1] & 0xffff0000u : w[r][k >> 1] << 16); }
+  __device__ __forceinline__ uint32_t magnitudes(int r, int k) const { return w[r][k] & 0x7fff7fffu; }
+  __device__ __forceinline__ uint32_t row_top(int r) const {
+    const uint32_t t = __vimax3_u16x2(__vimax3_u16x2(magnitudes(r, 0), magnitudes(r, 1), magnitudes(r, 2)), magnitudes(r, 3), 0u);
+    return max(t << 16, t & 0xffff0000u);
+  }
+  __device__ __forceinline__ void column_tops(uint32_t (&down)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t t = magnitudes(0, k);
+#pragma unroll
+      for (int r = 1; r < 7; r += 2) t = __vimax3_u16x2(t, magnitudes(r, k), magnitudes(r + 1, k));
+      t = __vimax3_u16x2(t, magnitudes(7, k), 0u);
+      t = __vimax3_u16x2(t, __shfl_xor_sync(0xffffffffu, t, 16), 0u);
+      down[2 * k] = t << 16;
+      down[2 * k + 1] = t & 0xffff0000u;
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint2 row_bytes(const Patch<T>& x, int r, float f) {
+  const float v[8] = {x.at(r, 0), x.at(r, 1), x.at(r, 2), x.at(r, 3), x.at(r, 4), x.at(r, 5), x.at(r, 6), x.at(r, 7)};
+  return e4m3x8(v, f);
+}
+
 // A CTA takes a 128 x 128 tile: thread (ty, tx) holds rows 8 ty .. 8 ty + 7 and columns 8 tx .. 8 tx + 7.  The transpose goes through
 // shared memory, where a thread has eight neighbouring bytes of each of its columns; piece p of row c lies at p ^ (c / 8), so that the
 // threads of a row of tiles write to different banks.
 constexpr int kTileThreads = 256;
 
 template <typename T, bool kVec, bool kSquares>
-__global__ void __launch_bounds__(kTileThreads, 2)
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 3 : 2)
 fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale, uint8_t* __restrict__ qt,
                 long long ldt, float* __restrict__ scale_t, long long rows, int K) {
   __shared__ __align__(16) uint32_t col_top[kTileThreads / 32][kFp8Group];
@@ -119,19 +190,15 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
   const long long tb = blockIdx.y;
   const int col = kb * kFp8Group + tx * 8;
   const long long row0 = tb * kFp8Group + ty * 8;
-  float v[8][8];
+  Patch<T> v;
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    if (row0 + r < rows) {
-      load8<kVec>(x + (row0 + r) * ldx, col, K, v[r]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[r][k] = 0.f;
-    }
+    if (row0 + r < rows) v.template load<kVec>(r, x + (row0 + r) * ldx, col, K);
+    else v.clear(r);
   }
   uint32_t tops[8];  // of a thread's rows
 #pragma unroll
-  for (int r = 0; r < 8; ++r) tops[r] = top_of(v[r]);
+  for (int r = 0; r < 8; ++r) tops[r] = v.row_top(r);
   float factor_t[8];
   if constexpr (kSquares) {
     uint32_t t = 0;
@@ -150,17 +217,11 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
     if (threadIdx.x == 0) scale[tb * gridDim.x + kb] = s.scale;
 #pragma unroll
     for (int r = 0; r < 8; ++r)
-      if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = e4m3x8(v[r], s.factor);
+      if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = row_bytes(v, r, s.factor);
     if (qt == nullptr) return;
   } else {
     uint32_t down[8];  // of a thread's columns, with the other eight rows of the warp
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t t = 0;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) t = max(t, magnitude_bits(v[r][k]));
-      down[k] = max(t, __shfl_xor_sync(0xffffffffu, t, 16));
-    }
+    v.column_tops(down);
     if ((threadIdx.x & 16) == 0) {
       *reinterpret_cast<uint4*>(&col_top[warp][tx * 8]) = make_uint4(down[0], down[1], down[2], down[3]);
       *reinterpret_cast<uint4*>(&col_top[warp][tx * 8 + 4]) = make_uint4(down[4], down[5], down[6], down[7]);
@@ -170,7 +231,7 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const float factor = __shfl_sync(0xffffffffu, mine.factor, (threadIdx.x & 16) + 2 * r);
-      if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = e4m3x8(v[r], factor);
+      if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = row_bytes(v, r, factor);
     }
     __syncthreads();
     if (threadIdx.x < kFp8Group) {
@@ -188,7 +249,7 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float c[8] = {v[0][k], v[1][k], v[2][k], v[3][k], v[4][k], v[5][k], v[6][k], v[7][k]};
+    const float c[8] = {v.at(0, k), v.at(1, k), v.at(2, k), v.at(3, k), v.at(4, k), v.at(5, k), v.at(6, k), v.at(7, k)};
     *reinterpret_cast<uint2*>(flipped + (tx * 8 + k) * kFp8Group + (ty ^ tx) * 8) = e4m3x8(c, factor_t[k]);
   }
   __syncthreads();
@@ -881,7 +942,8 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
   };
   // The shape of a tile by what the product would take with it: waves of tiles times the time of one group step of a tile, in units of a step of 128 x 128
   // (measured on 16384 x 8192 x 2048: 269 us with pairs, 326 with 128 x 128, 644 with 128 x 64; a scale per row of B: 482, 499 as pairs of 256 x 128,
-  // 695).  Tiles of single CTAs are cut along K among up to eight while SMs are idle; joining them takes about two steps.
+  // 695).  Tiles of single CTAs are cut along K among up to eight while SMs are idle; joining two or
+  // four takes about two steps, eight (which have to start on one GPC) about twelve.
   auto with_n = [&](auto column, auto out_tag) {
     constexpr bool kColumn = decltype(column)::value;
     auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
@@ -893,7 +955,7 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
     for (int n : {64, 128}) {
       const int64_t tiles = up(M, 128) * up(N, n);
       for (int s = n == 64 ? 1 : 2; s <= kMaxSplits && (s == 1 || (tiles * s <= sms && p.groups >= 2 * s)); s *= 2) {
-        const double t = up(tiles * s, sms) * (n == 64 ? narrow_step : 1.) * up(p.groups, s) + (s > 1 ? 2. : 0.);
+        const double t = up(tiles * s, sms) * (n == 64 ? narrow_step : 1.) * up(p.groups, s) + (s == 8 ? 12. : s > 1 ? 2. : 0.);
         if (t < best) {
           best = t;
           cut_n = n;

@@ -202,12 +202,30 @@ std::vector<Tensor> fp8_linear(const Tensor& x, const std::vector<Tensor>& weigh
   return Fp8Linear::apply(x, at::TensorList(weights), out_bf16, status, learns);
 }
 
+// x [..., K] with weights that are held in 8 bits (e4m3 bytes [N_i, K], rows at multiples of 16 bytes, scales per square); no gradient.
+std::vector<Tensor> fp8_linear_held(const Tensor& x, const std::vector<Tensor>& data, const std::vector<Tensor>& scales, bool out_bf16, const Tensor& status) {
+  TORCH_CHECK(data.size() == scales.size(), "fp8: a scale for every weight");
+  torch::NoGradGuard no_grad;
+  const int64_t K = x.size(-1);
+  auto [q, s] = fp8_rows(x.reshape({-1, K}).contiguous());
+  ++launches;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  std::vector<Tensor> out;
+  for (size_t i = 0; i < data.size(); ++i) {
+    sizes.back() = data[i].size(0);
+    out.push_back(fp8_matmul(bytes(q, K), s.t(), data[i].view(torch::kUInt8), scales[i], false, out_bf16, std::nullopt, status, sizes));
+    ++launches;
+  }
+  return out;
+}
+
 void register_model_autograd(pybind11::module_& m) {
   namespace py = pybind11;
   const auto unlocked = py::call_guard<py::gil_scoped_release>();
   m.def("add_rms_norm", &add_rms_norm, unlocked);
   m.def("embedding", &embedding, unlocked);
   m.def("fp8_linear", &fp8_linear, unlocked);
+  m.def("fp8_linear_held", &fp8_linear_held, unlocked);
   m.def("model_op_launches", [] { return launches.load(); });
 }
 

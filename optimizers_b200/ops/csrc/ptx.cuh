@@ -304,8 +304,8 @@ __device__ __forceinline__ void tmem_ld_32_issue(uint32_t taddr, uint32_t (&r)[3
       : "memory");
 }
 
-// 16 lanes x 2 n fp32 columns into n registers, not waited for: thread t receives in 2 i the value of row t / 4 and in 2 i + 1 that of row
-// t / 4 + 8, both of column 4 i + t % 4.
+// 16 lanes x 32 fp32 columns, not waited for: thread t receives in 2 i the value of row t / 4 and in 2 i + 1 that of row t / 4 + 8, both of
+// column 4 i + t % 4.
 __device__ __forceinline__ void tmem_ld_16_issue(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x128b.x8.b32 "
@@ -315,19 +315,6 @@ __device__ __forceinline__ void tmem_ld_16_issue(uint32_t taddr, uint32_t (&r)[1
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_16_issue(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x128b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-
 // Waits for every load that the thread has issued.  `gate` passes through: a use of the loaded registers that also needs the gate cannot move
 // ahead of the wait.  (Passing the registers themselves through costs a move for most of them.)
 __device__ __forceinline__ void tmem_ld_wait(uint64_t& gate) {

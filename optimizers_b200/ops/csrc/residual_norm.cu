@@ -251,8 +251,6 @@ void with_shape(const NormShape& s, bool vec, F&& f) {
 
 }  // namespace
 
-int64_t add_norm_max_width() { return kMaxNormWidth; }
-
 // x, r [..., C] (r may be absent; fp32 x with bf16 r is not offered) -> (y, scale, h, rstd).  out: 0 fp32, 1 bf16, 2 e4m3 (uint8, rows at a
 // pitch of a multiple of 16 bytes) with scale [groups, rows].  h is empty where r is absent (it is x then).
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> add_norm_fwd(const torch::Tensor& x, const std::optional<torch::Tensor>& r,
@@ -332,7 +330,6 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> add_norm_bwd(const torch
 }
 
 void register_residual_norm_ops(pybind11::module_& m) {
-  m.def("add_norm_max_width", &add_norm_max_width);
   m.def("add_norm_fwd", &add_norm_fwd);
   m.def("add_norm_bwd", &add_norm_bwd);
 }

@@ -52,12 +52,22 @@ def test_linear_with_several_weights_and_held_operands():
         assert fp8.linear(fp8.quantize_rows(x), ws[0]).dtype == BF16
 
 
+def test_linear_without_rows():
+    w = torch.randn(4, 5, requires_grad=True)
+    y = fp8.linear(torch.randn(0, 5, requires_grad=True), w)
+    y.sum().backward()
+    assert y.shape == (0, 4) and not w.grad.any()
+
+
 def test_refusals_of_linear():
     x, w = torch.randn(4, 130), torch.randn(6, 130)
     with pytest.raises(ValueError, match="fit"):
         fp8.linear(x, torch.randn(6, 131))
     with pytest.raises(ValueError, match="weight"):
         fp8.linear(x, ())
+    for empty in (torch.randn(4, 0), torch.tensor(1.0)):
+        with pytest.raises(ValueError, match="at least one value"):
+            fp8.linear(empty, torch.randn(6, 0))
     with pytest.raises(ValueError, match="floating"):
         fp8.linear(x, w, out_dtype=torch.int32)
     with pytest.raises(ValueError, match="floating"):
@@ -97,7 +107,7 @@ def test_add_rms_norm(kinds):
 
 def test_refusals_of_add_rms_norm():
     x, w = torch.randn(3, 16), torch.randn(16)
-    for bad in ((x, x[:2], w), (x, x, w[:8]), (x, None, w), (x.long(), x, w)):
+    for bad in ((x, x[:2], w), (x, x, w[:8]), (x[:, :0], x[:, :0], w[:0]), (x, None, w), (x.long(), x, w)):
         with pytest.raises(ValueError):
             fused_ops.add_rms_norm(*bad)
     with pytest.raises(ValueError, match="no gradient"):

@@ -32,6 +32,23 @@ def _full(q, scale, down):
     return q * scale.double().repeat_interleave(down, 0)[: q.shape[0]].repeat_interleave(128, 1)[:, : q.shape[1]]
 
 
+def _both(x):
+    """Both layouts from the kernel: ((values, scales), (values, scales of the transpose))."""
+    raw, scale, raw_t, scale_t = fused_ops._ext().fp8_both(x)
+    return (fp8._e4m3(raw, x.shape[1]), scale.t()), (fp8._e4m3(raw_t, x.shape[0]), scale_t.t())
+
+
+def _squares(w):
+    raw, raw_t, scale = fused_ops._ext().fp8_squares(w, True)
+    return (fp8._e4m3(raw, w.shape[1]), scale), (fp8._e4m3(raw_t, w.shape[0]), scale.t())
+
+
+def _product(a, b, column, out, addend=None):
+    return fused_ops._ext().fp8_matmul(
+        a[0].view(torch.uint8), a[1], b[0].view(torch.uint8), b[1], column, out == BF16, addend, fp8._status_of(a[0].device)
+    )
+
+
 SHAPES = [(1, 1), (1, 16), (3, 127), (5, 128), (7, 129), (128, 128), (127, 300), (129, 256), (257, 1000), (300, 1337)]
 
 
@@ -42,12 +59,12 @@ def test_formats_are_the_definition_bit_for_bit(shape, dtype):
     q, s = _held(x, 1)
     rows = fp8.quantize_rows(x)
     assert torch.equal(rows.scale, s) and torch.equal(rows.data.double(), q)
-    (a, sa), (b, sb) = fp8._both(x, True)
+    (a, sa), (b, sb) = _both(x)
     assert torch.equal(sa, s) and torch.equal(a.double(), q)
     qt, st = _held(x.t(), 1)
     assert torch.equal(sb, st) and torch.equal(b.double(), qt)
     qw, sw = _held(x, 128)
-    (c, sc), (d, sd) = fp8._squares(x, True, True)
+    (c, sc), (d, sd) = _squares(x)
     assert torch.equal(sc, sw) and torch.equal(c.double(), qw)
     assert torch.equal(sd, sw.t()) and torch.equal(d.double(), qw.t())
     w = fp8.quantize_weight(x)
@@ -60,7 +77,8 @@ def test_formats_of_strided_unaligned_and_extreme_sources(dtype):
     for view in (wide[:, 3:300], wide[:, 8:264], wide[::2, :256], wide.t(), wide[5:6, 1:2]):
         for got, want in zip(fp8._rows(view, True), fp8._rows(view.contiguous(), True)):
             assert torch.equal(got.float(), want.float())
-        for got, want in zip(fp8._both(view, True), fp8._both(view.contiguous(), True)):
+        source = fp8._source(view)
+        for got, want in zip(_both(source), _both(view.contiguous())):
             assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
     x = torch.zeros(4, 256, device="cuda", dtype=dtype)
     x[1, :128] = 1e-38
@@ -78,9 +96,9 @@ def test_formats_of_strided_unaligned_and_extreme_sources(dtype):
 
 def _product_case(M, N, K, column, out, addend, seed=0):
     a, sa = fp8._rows(_x(M, K, F32, seed), True)
-    b, sb = fp8._rows(_x(N, K, F32, seed + 1), True) if column else fp8._squares(_x(N, K, F32, seed + 1), False, True)[0]
+    b, sb = fp8._rows(_x(N, K, F32, seed + 1), True) if column else fp8._squares(_x(N, K, F32, seed + 1), True)
     add = _x(M, N, F32, seed + 2) if addend else None
-    got = fp8._product((a, sa), (b, sb), column, out, True, add)
+    got = _product((a, sa), (b, sb), column, out, add)
     fa, fb = _full(a.double(), sa, 1), _full(b.double(), sb, 1 if column else 128)
     want = fa @ fb.t() + (add.double() if addend else 0)
     size = fa.abs() @ fb.abs().t() + (add.double().abs() if addend else 0)
@@ -307,3 +325,41 @@ def test_llama_runs_all_of_it_together():
     model.train()
     assert all(layer._held is None for layer in model.layers)
     fp8.check_status()
+
+
+def test_inference_mode_and_another_current_device_state():
+    x, w, r = _x(20, 256), _x(64, 256, F32, 1), _x(20, 256, F32, 2)
+    weight, table, ids = torch.ones(256, device="cuda"), _x(30, 16, F32), torch.arange(10, device="cuda")
+    with torch.inference_mode():
+        y = fp8.linear(x, (w, w))[1]
+        n, h = fused_ops.add_rms_norm(x, r, weight)
+        rows, h8 = fp8.add_rms_norm(x, r, weight)
+        e = fused_ops.embedding(ids, table)
+        z = fp8.linear(rows, fp8.quantize_weight(w))
+    with torch.no_grad():
+        assert torch.equal(y, fp8.linear(x, w)) and torch.equal(h, h8) and torch.equal(e, table[:10])
+        m, k = fused_ops.add_rms_norm(x, r, weight)
+        assert torch.equal(n, m) and torch.equal(h, k)
+        assert torch.equal(z, fp8.linear(rows, w))
+
+
+def test_differentiating_a_gradient_again_is_refused():
+    x, w = _x(9, 130, F32).requires_grad_(), _x(20, 130, F32, 1).requires_grad_()
+    r, n, table = _x(9, 130, F32, 2).requires_grad_(), torch.ones(130, device="cuda", requires_grad=True), _x(30, 16, F32).requires_grad_()
+    for out, leaf in (
+        (fp8.linear(x, w), x), (fused_ops.add_rms_norm(x, r, n)[0], x), (fused_ops.embedding(torch.arange(4, device="cuda"), table), table)
+    ):
+        (g,) = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="again"):
+            g.sum().backward()
+        with pytest.raises(RuntimeError):  # (nothing leads from the gradient back to the leaf)
+            torch.autograd.grad(g.sum(), leaf)
+
+
+def test_in_place_changes_of_what_the_backward_pass_needs_are_found():
+    x, r, n = _x(9, 128, F32).requires_grad_(), _x(9, 128, F32, 1).requires_grad_(), torch.ones(128, device="cuda", requires_grad=True)
+    y, h = fused_ops.add_rms_norm(x, r, n)
+    with torch.no_grad():
+        h += 1.0
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
