@@ -11,13 +11,17 @@
 //              of the batch costs no more than others.  A token whose pairs lie in one piece goes straight into the table; the
 //              others leave a partial sum per piece.
 //   3. joins   adds the partial sums of a token in the order of the pieces.
-// Up to 64 tokens take one launch instead.
-// No floating-point atomics: the same inputs give the same bits.
+// Up to 128 tokens take one launch instead.
+// No floating-point atomics: the same inputs give the same bits.  16384 tokens over 50257 x 768 fp32: 27 + 14 + 11 us; the write of the table alone
+// takes 24.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <torch/extension.h>
+
+#include <map>
+#include <mutex>
 
 #include "ptx.cuh"
 
@@ -50,7 +54,7 @@ __device__ __forceinline__ long long token_at(const Id* ids, long long i) {
 
 // ------------------------------------------------------------------------------------------------
 // Forward: bound by HBM and the L2 (rows of frequent tokens stay there).  A warp takes 128 packs of one row, four loads in
-// flight per lane.  A token outside the table gives a row of NaN.
+// flight per lane.  A token outside the table gives a row of NaN.  16384 x 768 fp32: 16 us (6.1 TB/s).
 // ------------------------------------------------------------------------------------------------
 template <int N, typename T, typename Out, typename Id>
 __global__ void __launch_bounds__(256)
@@ -322,16 +326,18 @@ embed_join_kernel(const unsigned* __restrict__ keys, const float* __restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------
-// Up to 64 tokens: one launch, a warp per row of the table and 128 packs of it, which looks the row's number up among the tokens.  The
+// Up to 128 tokens: one launch, a warp per row of the table and 128 packs of it, which looks the row's number up among the tokens.  The
 // three launches of the sort would cost more than the sums; beyond this the longest sum (one token throughout) would.
 // ------------------------------------------------------------------------------------------------
-constexpr int kFewTokens = 64;
+constexpr int kFewTokens = 128;
 
 template <int N, typename Grad, typename T, typename Id>
 __global__ void __launch_bounds__(256)
 embed_few_kernel(const Id* __restrict__ ids, const Grad* __restrict__ dy, T* __restrict__ table, int n, long long V, int C, float scale) {
   const int packs = C / N, segs = (packs + 127) / 128, lane = threadIdx.x & 31;
-  const long long mine[2] = {lane < n ? token_at(ids, lane) : -1, lane + 32 < n ? token_at(ids, lane + 32) : -1};
+  long long mine[kFewTokens / 32];
+#pragma unroll
+  for (int h = 0; h < kFewTokens / 32; ++h) mine[h] = h * 32 + lane < n ? token_at(ids, h * 32 + lane) : -1;
   const long long items = V * segs, step = static_cast<long long>(gridDim.x) * 8;
   for (long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < items; w += step) {
     const long long v = w / segs;
@@ -342,22 +348,28 @@ embed_few_kernel(const Id* __restrict__ ids, const Grad* __restrict__ dy, T* __r
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[q][k] = 0.f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      unsigned who = __ballot_sync(0xffffffffu, mine[half] == v);
-      while (who != 0) {  // in ascending order
-        const int t = half * 32 + __ffs(who) - 1;
+    for (int h = 0; h < kFewTokens / 32; ++h) {
+      unsigned who = __ballot_sync(0xffffffffu, mine[h] == v);
+      while (who != 0) {  // in ascending order, two rows on their way at a time
+        int t[2];
+        t[0] = h * 32 + __ffs(who) - 1;
         who &= who - 1;
-        const auto* src = reinterpret_cast<const Pack<N, Grad>*>(dy + static_cast<long long>(t) * C);
-        Pack<N, Grad> u[4];
+        t[1] = who != 0 ? h * 32 + __ffs(who) - 1 : -1;
+        who &= who - 1;
+        Pack<N, Grad> u[2][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (first + 32 * q < packs) u[q] = src[first + 32 * q];
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (first + 32 * q < packs) {
+          for (int q = 0; q < 4; ++q)
+            if (t[r] >= 0 && first + 32 * q < packs) u[r][q] = reinterpret_cast<const Pack<N, Grad>*>(dy + static_cast<long long>(t[r]) * C)[first + 32 * q];
 #pragma unroll
-            for (int k = 0; k < N; ++k) acc[q][k] += as_float(u[q].e[k]);
-          }
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (t[r] >= 0 && first + 32 * q < packs) {
+#pragma unroll
+              for (int k = 0; k < N; ++k) acc[q][k] += as_float(u[r][q].e[k]);
+            }
       }
     }
 #pragma unroll
@@ -368,6 +380,33 @@ embed_few_kernel(const Id* __restrict__ ids, const Grad* __restrict__ dy, T* __r
       store_row<N, T, false>(table, v * C + static_cast<long long>(first + 32 * q) * N, acc[q]);
     }
   }
+}
+
+// Clusters of the sort kernel that the device holds at once: the zeros are shared out among those, since a cluster of a second wave would double
+// their time (18 clusters of eight are one per SM of 148, but 16 fit into the GPCs: 41 us instead of 27 for 50257 x 768).
+template <typename Kernel>
+int clusters_at_once(Kernel* kernel, size_t smem) {
+  static std::mutex mutex;
+  static std::map<std::pair<const void*, int>, int> known;
+  int device = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mutex);
+  int& n = known[{reinterpret_cast<const void*>(kernel), device}];
+  if (n == 0) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kSortCtas);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {kSortCtas, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    n = std::max(n, 2);
+  }
+  return n;
 }
 
 bool fp32_or_bf16(const torch::Tensor& t) { return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16; }
@@ -481,14 +520,13 @@ torch::Tensor embed_bwd(const torch::Tensor& ids, const torch::Tensor& dy, int64
   for (int64_t i0 = 0; i0 < n; i0 += kSortCapacity) {
     const int count = static_cast<int>(std::min<int64_t>(kSortCapacity, n - i0));
     const int64_t bytes = i0 == 0 ? out.numel() * out.element_size() : 0, vecs = bytes / 16;
-    const int zero_ctas = static_cast<int>(std::min<int64_t>((sms - kSortCtas) / kSortCtas, (bytes + 8 * kZeroBytes - 1) / (8 * kZeroBytes))) * kSortCtas;
     const int per = count <= kSortCtas * kSortThreads ? 1 : count <= 2 * kSortCtas * kSortThreads ? 2 : count <= 4 * kSortCtas * kSortThreads ? 4 : 8;
     with_ids(ids, [&](auto* idp) {
       using Id = std::remove_cv_t<std::remove_pointer_t<decltype(idp)>>;
       auto sort = [&](auto kPer) {
         auto* kernel = embed_sort_kernel<decltype(kPer)::value, Id>;
         const size_t smem = sort_smem(decltype(kPer)::value);
-        if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        const int zero_ctas = static_cast<int>(std::min<int64_t>(clusters_at_once(kernel, smem) - 1, (bytes + 8 * kZeroBytes - 1) / (8 * kZeroBytes))) * kSortCtas;
         kernel<<<kSortCtas + zero_ctas, kSortThreads, smem, st>>>(
             idp + i0, count, V, bits, keys, pos,
             reinterpret_cast<uint4*>(out.data_ptr()), vecs, reinterpret_cast<unsigned char*>(out.data_ptr()) + vecs * 16, static_cast<int>(bytes - vecs * 16));

@@ -24,11 +24,9 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------
-// Into the format.  Bound by HBM: one read of x, one byte written per value and operand.
+// Into the format.  Bound by HBM: one read of x, one byte written per value and operand.  bf16, 16384 x 8192: rows 72 us (5.6 TB/s), both
+// layouts 96 us (5.6 TB/s); fp32 8192 x 2048 into squares and their transpose 23 us (4.5 TB/s).
 // ------------------------------------------------------------------------------------------------
-constexpr int kRowsThreads = 256;
-constexpr int kRowsAtOnce = 4;  // groups of sixteen lanes in flight
-
 __device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
   uint32_t top = 0;
 #pragma unroll
@@ -53,53 +51,6 @@ __device__ __forceinline__ uint32_t spread_max(uint32_t (&v)[kCount], int lane) 
 #pragma unroll
   for (; o > 0; o >>= 1) v[0] = max(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
   return v[0];
-}
-
-// Sixteen lanes take four groups, eight values each of every group.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowsThreads)
-fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale, long long rows, int K) {
-  const int groups = (K + kFp8Group - 1) / kFp8Group, lane = threadIdx.x & 15;
-  const long long total = rows * groups;
-  const long long first = ((static_cast<long long>(blockIdx.x) * kRowsThreads + threadIdx.x) >> 4) * kRowsAtOnce;
-  float v[kRowsAtOnce][8];
-  long long row = first / groups;
-  int kb = static_cast<int>(first - row * groups);
-  const long long row0 = row;
-  const int kb0 = kb;
-  uint32_t top[kRowsAtOnce];
-#pragma unroll
-  for (int i = 0; i < kRowsAtOnce; ++i) {
-    if (first + i < total) {
-      load8<kVec>(x + row * ldx, kb * kFp8Group + lane * 8, K, v[i]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
-    }
-    if (++kb == groups) {
-      kb = 0;
-      ++row;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kRowsAtOnce; ++i) top[i] = top_of(v[i]);
-  const GroupScale s = group_scale(spread_max(top, lane));
-  row = row0;
-  kb = kb0;
-#pragma unroll
-  for (int i = 0; i < kRowsAtOnce; ++i) {
-    const int from = (threadIdx.x & 16) + i * (16 / kRowsAtOnce);
-    const float factor = __shfl_sync(0xffffffffu, s.factor, from), held = __shfl_sync(0xffffffffu, s.scale, from);
-    if (first + i < total) {
-      const int col = kb * kFp8Group + lane * 8;
-      if (col < K) *reinterpret_cast<uint2*>(q + row * ldq + col) = e4m3x8(v[i], factor);  // the pitch is a multiple of 16
-      if (lane == 0) scale[static_cast<long long>(kb) * rows + row] = held;
-    }
-    if (++kb == groups) {
-      kb = 0;
-      ++row;
-    }
-  }
 }
 
 // Eight rows of eight neighbouring values as a thread of the tile kernel holds them.  bf16 stays packed: half the registers, and
@@ -173,12 +124,14 @@ __device__ __forceinline__ uint2 row_bytes(const Patch<T>& x, int r, float f) {
   return e4m3x8(v, f);
 }
 
+enum TileFormat { kRowGroups, kBothGroups, kSquareGroups };
+
 // A CTA takes a 128 x 128 tile: thread (ty, tx) holds rows 8 ty .. 8 ty + 7 and columns 8 tx .. 8 tx + 7.  The transpose goes through
 // shared memory, where a thread has eight neighbouring bytes of each of its columns; piece p of row c lies at p ^ (c / 8), so that the
 // threads of a row of tiles write to different banks.
 constexpr int kTileThreads = 256;
 
-template <typename T, bool kVec, bool kSquares>
+template <typename T, bool kVec, TileFormat kFormat>
 __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 3 : 2)
 fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale, uint8_t* __restrict__ qt,
                 long long ldt, float* __restrict__ scale_t, long long rows, int K) {
@@ -200,7 +153,7 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
 #pragma unroll
   for (int r = 0; r < 8; ++r) tops[r] = v.row_top(r);
   float factor_t[8];
-  if constexpr (kSquares) {
+  if constexpr (kFormat == kSquareGroups) {
     uint32_t t = 0;
 #pragma unroll
     for (int r = 0; r < 8; ++r) t = max(t, tops[r]);
@@ -220,11 +173,13 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
       if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = row_bytes(v, r, s.factor);
     if (qt == nullptr) return;
   } else {
-    uint32_t down[8];  // of a thread's columns, with the other eight rows of the warp
-    v.column_tops(down);
-    if ((threadIdx.x & 16) == 0) {
-      *reinterpret_cast<uint4*>(&col_top[warp][tx * 8]) = make_uint4(down[0], down[1], down[2], down[3]);
-      *reinterpret_cast<uint4*>(&col_top[warp][tx * 8 + 4]) = make_uint4(down[4], down[5], down[6], down[7]);
+    if constexpr (kFormat == kBothGroups) {
+      uint32_t down[8];  // of a thread's columns, with the other eight rows of the warp
+      v.column_tops(down);
+      if ((threadIdx.x & 16) == 0) {
+        *reinterpret_cast<uint4*>(&col_top[warp][tx * 8]) = make_uint4(down[0], down[1], down[2], down[3]);
+        *reinterpret_cast<uint4*>(&col_top[warp][tx * 8 + 4]) = make_uint4(down[4], down[5], down[6], down[7]);
+      }
     }
     const GroupScale mine = group_scale(spread_max(tops, tx));  // of row tx / 2
     if ((tx & 1) == 0 && row0 + tx / 2 < rows) scale[static_cast<long long>(kb) * rows + row0 + tx / 2] = mine.scale;
@@ -233,6 +188,7 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
       const float factor = __shfl_sync(0xffffffffu, mine.factor, (threadIdx.x & 16) + 2 * r);
       if (row0 + r < rows && col < K) *reinterpret_cast<uint2*>(q + (row0 + r) * ldq + col) = row_bytes(v, r, factor);
     }
+    if constexpr (kFormat == kRowGroups) return;
     __syncthreads();
     if (threadIdx.x < kFp8Group) {
       uint32_t t = 0;
@@ -275,8 +231,14 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
 // arrangement at 124 (column pairs of eight rows would come at 64); the fp32 units take one operation per clock.  So the epilogue needs about
 // 256 or 512 clocks per group of a 128 x 256 tile, next to 512 of the MMAs.  The next piece of a buffer is on its way while one is added.
 //
-// Large products are computed by pairs of CTAs, 256 x 256 results each: with 128 x 256 per CTA the loads from the L2 (48 KB per group and SM, 11.5
-// TB/s over the chip) bound the kernel at half of the tensor rate whatever the epilogue does; a pair loads 32 KB per group and SM.
+// Large products are computed by pairs of CTAs, 256 x 256 results each.  With 128 x 256 per CTA a group moves 48 KB into shared memory and
+// 48 KB from there to the tensor cores, 768 clocks of 128 bytes for 512 of MMAs; a pair moves 32 and 32 KB per SM.
+//
+// What bounds it: the epilogue, about 950 clocks per group, of which 256 are multiply-adds (two warps per scheduler that run in step) and the
+// rest TMEM loads, barriers and their latencies; with a scale per row of B about 1550.  16384 x 2048 x 8192 by pairs: 160 us without
+// an epilogue, 184 without the multiply-adds, 242 as it is (2.27 PFLOP/s; 1.62 for the bf16 library product); 8192 x 16384 x 2048 with a
+// scale per row of B 397 us (1.38 PFLOP/s), 242 without the multiply-adds.  Sixteen epilogue warps with half the columns each spill
+// (429 us); reading TMEM as column pairs of eight rows took 305 us, single CTAs of 128 x 256 265 us.
 //
 // Products with few tiles are cut along K among the CTAs of a cluster, whose partial sums meet in distributed shared memory: each CTA adds
 // the sums of all ranks, in rank order, for its share of the tile.
@@ -837,13 +799,12 @@ std::tuple<torch::Tensor, torch::Tensor> fp8_rows(const torch::Tensor& x) {
   auto q = bytes_of(x, T, K);
   auto scale = torch::empty({G, T}, x.options().dtype(torch::kFloat32));
   if (T == 0 || K == 0) return {q, scale};
-  const int64_t sets = (T * G + kRowsAtOnce - 1) / kRowsAtOnce, grid = (sets * 16 + kRowsThreads - 1) / kRowsThreads;
-  TORCH_CHECK(grid < (1LL << 31), "fp8: the source is too large");
+  TORCH_CHECK(groups_of(T) <= 65535, "fp8: the source has too many rows");
   auto st = at::cuda::getCurrentCUDAStream();
   with_source(x, [&](auto* p, auto vec) {
     using T_ = std::remove_cv_t<std::remove_pointer_t<decltype(p)>>;
-    fp8_rows_kernel<T_, decltype(vec)::value><<<static_cast<unsigned>(grid), kRowsThreads, 0, st>>>(
-        p, x.stride(0), q.data_ptr<uint8_t>(), q.stride(0), scale.data_ptr<float>(), T, static_cast<int>(K));
+    fp8_tile_kernel<T_, decltype(vec)::value, kRowGroups><<<dim3(static_cast<unsigned>(G), static_cast<unsigned>(groups_of(T))), kTileThreads, 0, st>>>(
+        p, x.stride(0), q.data_ptr<uint8_t>(), q.stride(0), scale.data_ptr<float>(), nullptr, 0, nullptr, T, static_cast<int>(K));
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {q, scale};
@@ -862,7 +823,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> fp8_both(
   auto st = at::cuda::getCurrentCUDAStream();
   with_source(x, [&](auto* p, auto vec) {
     using T_ = std::remove_cv_t<std::remove_pointer_t<decltype(p)>>;
-    fp8_tile_kernel<T_, decltype(vec)::value, false><<<dim3(static_cast<unsigned>(G), static_cast<unsigned>(H)), kTileThreads, 0, st>>>(
+    fp8_tile_kernel<T_, decltype(vec)::value, kBothGroups><<<dim3(static_cast<unsigned>(G), static_cast<unsigned>(H)), kTileThreads, 0, st>>>(
         p, x.stride(0), q.data_ptr<uint8_t>(), q.stride(0), scale.data_ptr<float>(), qt.data_ptr<uint8_t>(), qt.stride(0), scale_t.data_ptr<float>(), T,
         static_cast<int>(K));
   });
@@ -882,7 +843,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> fp8_squares(const torch:
   auto st = at::cuda::getCurrentCUDAStream();
   with_source(w, [&](auto* p, auto vec) {
     using T_ = std::remove_cv_t<std::remove_pointer_t<decltype(p)>>;
-    fp8_tile_kernel<T_, decltype(vec)::value, true><<<dim3(static_cast<unsigned>(G), static_cast<unsigned>(H)), kTileThreads, 0, st>>>(
+    fp8_tile_kernel<T_, decltype(vec)::value, kSquareGroups><<<dim3(static_cast<unsigned>(G), static_cast<unsigned>(H)), kTileThreads, 0, st>>>(
         p, w.stride(0), q.data_ptr<uint8_t>(), q.stride(0), scale.data_ptr<float>(), transpose ? qt.data_ptr<uint8_t>() : nullptr, qt.stride(0), nullptr, N,
         static_cast<int>(K));
   });

@@ -59,6 +59,13 @@ def test_linear_without_rows():
     assert y.shape == (0, 4) and not w.grad.any()
 
 
+def test_first_use_inside_a_capture_is_refused(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(fp8, "_status", {})
+    with pytest.raises(RuntimeError, match="before capturing"):
+        fp8._status_of(torch.device("cpu"))
+
+
 def test_refusals_of_linear():
     x, w = torch.randn(4, 130), torch.randn(6, 130)
     with pytest.raises(ValueError, match="fit"):

@@ -49,7 +49,7 @@ def _check(ids, V, C, dtype, out, scale, seed=0, known=None):
     return table.grad
 
 
-@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 1000, 8192, 8193, 20000, 40000])
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 65, 127, 128, 129, 1000, 8192, 8193, 20000, 40000])
 @pytest.mark.parametrize("kind", ["uniform", "skewed", "same", "ramp"])
 def test_lengths_and_distributions(n, kind):
     V = 1000

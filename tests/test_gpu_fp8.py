@@ -327,7 +327,7 @@ def test_llama_runs_all_of_it_together():
     fp8.check_status()
 
 
-def test_inference_mode_and_another_current_device_state():
+def test_inference_mode():
     x, w, r = _x(20, 256), _x(64, 256, F32, 1), _x(20, 256, F32, 2)
     weight, table, ids = torch.ones(256, device="cuda"), _x(30, 16, F32), torch.arange(10, device="cuda")
     with torch.inference_mode():
