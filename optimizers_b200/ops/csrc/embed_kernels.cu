@@ -295,11 +295,10 @@ embed_join_kernel(const unsigned* __restrict__ keys, const float* __restrict__ p
   const unsigned token = keys[j * kPiece + kPiece - 1];
   if (token >= V || keys[(j + 1) * kPiece] != token) return;
   if (keys[j * kPiece] == token && j > 0 && keys[j * kPiece - 1] == token) return;  // it started earlier
-  int lo = j + 1, hi = pieces - 1;  // the last piece that begins with the token
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (keys[mid * kPiece] == token) lo = mid;
-    else hi = mid - 1;
+  int lo = j + 1;  // the last piece that begins with the token, looked for among as many as there are threads at a time
+  for (int more = 32 * kJoinRows; more == 32 * kJoinRows; lo += more) {
+    const int p = lo + 1 + static_cast<int>(threadIdx.x);
+    more = __syncthreads_count(p < pieces && keys[p * kPiece] == token);
   }
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   for (int c0 = blockIdx.y * 128; c0 < C; c0 += gridDim.y * 128) {

@@ -482,6 +482,11 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
       }
     }
+    if (warp == 0 && *abort_flag) {  // a pipeline that gave up leaves with no load of its own still on its way
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
     __syncwarp();
     if (!kPair && p.splits > 1) {
       cg::this_cluster().sync();
@@ -515,6 +520,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       constexpr int kPiece = kColumnScale || kN == 256 ? 32 : 16;                // columns
       constexpr int kPieces = kColumnScale ? 2 * kOwn / kPiece : kOwn / kPiece;  // upper and lower 16 rows apart where B has a scale per row
       constexpr int kQuarter = kPiece / 4;
+      static_assert(kPieces % 2 == 0, "the first piece of a group goes where the last one is not");
       uint32_t v[2][kColumnScale ? kPiece / 2 : kPiece];
       float scale[kRowsOwn], s[kColumnScale ? kQuarter : 1];
       const float* of_columns = nullptr;
@@ -574,7 +580,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (c + 2 == kPieces) look(true);
           } else {
             finish();
-            if (kPieces > 1 && g + 1 < g1) begin();
+            if (g + 1 < g1) begin();
           }
           if constexpr (!kColumnScale) {
 #pragma unroll
@@ -590,7 +596,6 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
           }
         }
-        if (kPieces == 1 && g + 1 < g1) begin();
       }
       ok = *abort_flag == 0;
       float acc[kOwn];  // the same, row by row: [column] or [row0 + 8 i][column of this lane]
