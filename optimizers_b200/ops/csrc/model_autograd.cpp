@@ -1,7 +1,7 @@
 // Autograd nodes of the decoder's operators.  They live here, not in Python, because a training step calls them hundreds of times: a Python
 // node costs 30 to 60 us of host time per call (forward and backward), as much as the kernels of a small model take.
 //
-// Gradients are first order: differentiating a gradient again raises an error.
+// Gradients are first order and taken one at a time: differentiating a gradient again, or a batch of incoming gradients, raises an error.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -31,8 +31,9 @@ std::atomic<int64_t> launches{0};
 
 bool is_bf16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16; }
 
-// fp32 or bf16, contiguous: what the kernels read.
+// fp32 or bf16, contiguous: what the kernels read.  (A batch of incoming gradients at once has no memory of its own to read.)
 Tensor readable(const Tensor& t) {
+  TORCH_CHECK(t.has_storage(), "this operator takes one gradient at a time, no batch of them (is_grads_batched, vmap)");
   return (t.scalar_type() == torch::kFloat32 || is_bf16(t) ? t : t.to(torch::kFloat32)).contiguous();
 }
 

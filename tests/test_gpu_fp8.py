@@ -363,3 +363,13 @@ def test_in_place_changes_of_what_the_backward_pass_needs_are_found():
         h += 1.0
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_batches_of_incoming_gradients_are_refused():
+    x, w = _x(9, 130, F32).requires_grad_(), _x(20, 130, F32, 1).requires_grad_()
+    r, n, table = _x(9, 130, F32, 2).requires_grad_(), torch.ones(130, device="cuda", requires_grad=True), _x(30, 16, F32).requires_grad_()
+    for out, leaf in (
+        (fp8.linear(x, w), x), (fused_ops.add_rms_norm(x, r, n)[0], x), (fused_ops.embedding(torch.arange(4, device="cuda"), table), table)
+    ):
+        with pytest.raises(RuntimeError, match="one gradient at a time"):
+            torch.autograd.grad(out, leaf, torch.ones(3, *out.shape, device="cuda"), is_grads_batched=True)
