@@ -586,13 +586,13 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
             for (int j = 0; j < kPiece / 2; ++j) {
               uint64_t& sum = sums[c * kPiece / 2 + j];
-              sum = fma2(pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), by, sum);
+              sum = fma2_loaded(v[c & 1][2 * j], v[c & 1][2 * j + 1], by, sum);
             }
           } else {
 #pragma unroll
             for (int i = 0; i < kQuarter; ++i) {
               uint64_t& sum = sums[(c & 1) * (kOwn / 4) + (c >> 1) * kQuarter + i];
-              sum = fma2(mul2(pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), by), pack2(s[i], s[i]), sum);
+              sum = fma2(mul2_loaded(v[c & 1][2 * i], v[c & 1][2 * i + 1], by), pack2(s[i], s[i]), sum);
             }
           }
         }

@@ -315,8 +315,9 @@ __device__ __forceinline__ void tmem_ld_16_issue(uint32_t taddr, uint32_t (&r)[1
       : "r"(taddr)
       : "memory");
 }
-// Waits for every load that the thread has issued.  `gate` passes through: a use of the loaded registers that also needs the gate cannot move
-// ahead of the wait.  (Passing the registers themselves through costs a move for most of them.)
+// Waits for every load that the thread has issued.  `gate` passes through: what is to happen after the wait takes it as an operand.  Loaded
+// registers are read by fma2_loaded and mul2_loaded only, whose one statement reads them and the gate, so that no read of them can move ahead
+// of the wait, not even the move that forms a pair.  (Passing the registers themselves through costs a move for most of them.)
 __device__ __forceinline__ void tmem_ld_wait(uint64_t& gate) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+l"(gate) : : "memory");
 }
@@ -339,9 +340,27 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+// Loaded registers (lo, hi) times the gate of their wait; and the same plus c.
+__device__ __forceinline__ uint64_t mul2_loaded(uint32_t lo, uint32_t hi, uint64_t gate) {
   uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  asm("{\n"
+      ".reg .b64 pair;\n"
+      "mov.b64 pair, {%1, %2};\n"
+      "mul.rn.f32x2 %0, pair, %3;\n"
+      "}\n"
+      : "=l"(d)
+      : "r"(lo), "r"(hi), "l"(gate));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2_loaded(uint32_t lo, uint32_t hi, uint64_t gate, uint64_t c) {
+  uint64_t d;
+  asm("{\n"
+      ".reg .b64 pair;\n"
+      "mov.b64 pair, {%1, %2};\n"
+      "fma.rn.f32x2 %0, pair, %3, %4;\n"
+      "}\n"
+      : "=l"(d)
+      : "r"(lo), "r"(hi), "l"(gate), "l"(c));
   return d;
 }
 
