@@ -632,19 +632,22 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         col = kColumnScale ? col0 + 16 * (j % (kOwn / 16)) + 4 * q : col0 + 4 * j;
       };
       if (!kPair && p.splits > 1) {
-        // The stages are idle: every load has arrived and every MMA is done.  [quad][thread]
+        // The stages are idle, every load has arrived and every MMA is done, unless this CTA gave up a wait: then a load that is still on its way may
+        // write over these sums, and the flag says so in their place.  [quad][thread]
         float4* mine = reinterpret_cast<float4*>(smem);
         const int thread = threadIdx.x - 32 * kFirstEpilogueWarp;
 #pragma unroll
         for (int j = 0; j < kOwn / 4; ++j) mine[j * 32 * kEpilogueWarps + thread] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
         cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
+        cluster.sync();  // behind the last wait of every warp
+        ok = __all_sync(0xffffffffu, *cluster.map_shared_rank(const_cast<int*>(abort_flag), min(lane, p.splits - 1)) == 0);
         for (int j = kOwn / 4 * rank / p.splits; j < kOwn / 4 * (rank + 1) / p.splits; ++j) {
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int r = 0; r < p.splits; ++r) {
             const float4 u = cluster.map_shared_rank(mine, r)[j * 32 * kEpilogueWarps + thread];
             sum.x += u.x; sum.y += u.y; sum.z += u.z; sum.w += u.w;
           }
+          if (!ok) sum.x = sum.y = sum.z = sum.w = __int_as_float(0x7fffffff);
           int row, col;
           place_quad(j, row, col);
           store_quad<Out>(p, row, col, sum);
