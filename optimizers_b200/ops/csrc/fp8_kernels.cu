@@ -9,10 +9,8 @@
 #include <cooperative_groups.h>
 #include <torch/extension.h>
 
-#include <mutex>
-#include <set>
-
 #include "fp8_format.cuh"
+#include "once.h"
 #include "ptx.cuh"
 #include "tensor_map.h"
 
@@ -720,18 +718,17 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // Once per kernel and device: room in shared memory, and that a kernel which moves registers between its warpgroups
 // has the registers at launch that it was written for (an increase beyond them would wait forever).
 void prepare_product(const void* kernel, int smem, int launch_regs) {
-  static std::mutex mutex;
-  static std::set<std::pair<const void*, int>> done;
+  static Once<std::pair<const void*, int>> once;
   int device = 0;
   C10_CUDA_CHECK(cudaGetDevice(&device));
-  std::lock_guard<std::mutex> lock(mutex);
-  if (!done.insert({kernel, device}).second) return;
-  if (launch_regs > 0) {
-    cudaFuncAttributes attr;
-    C10_CUDA_CHECK(cudaFuncGetAttributes(&attr, kernel));
-    TORCH_CHECK(attr.numRegs >= launch_regs, "fp8: the product was built with ", attr.numRegs, " registers per thread; it needs ", launch_regs);
-  }
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  once({kernel, device}, [&] {
+    if (launch_regs > 0) {
+      cudaFuncAttributes attr;
+      C10_CUDA_CHECK(cudaFuncGetAttributes(&attr, kernel));
+      TORCH_CHECK(attr.numRegs >= launch_regs, "fp8: the product was built with ", attr.numRegs, " registers per thread; it needs ", launch_regs);
+    }
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  });
 }
 
 // Results [M, N] in bf16, in boxes of 32 rows and 64 columns.
