@@ -266,8 +266,17 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.
         raise ValueError("embedding takes and returns floating-point tensors")
     if _kernels_take(weight) and type(ids) is torch.Tensor and ids.device == weight.device and out_dtype in _KINDS and weight.numel() > 0:
         return _ext().embedding(ids, weight, scale, out_dtype == torch.bfloat16)
-    y = F.embedding(ids, weight)
+    y = F.embedding(ids, weight) if ids.device.type == "cpu" else _embedding_of_known(ids, weight)
     return y.to(out_dtype) if scale == 1.0 else (y.float() * scale).to(out_dtype)
+
+
+def _embedding_of_known(ids: Tensor, weight: Tensor) -> Tensor:
+    """``weight[ids]`` with a row of NaN, without a gradient, for a token outside the table (PyTorch's lookup on a GPU would fault there)."""
+    nan = float("nan")
+    if weight.numel() == 0:  # no row to stand in
+        return weight.sum() + torch.full((*ids.shape, weight.shape[1]), nan, dtype=weight.dtype, device=weight.device)
+    known = (ids >= 0) & (ids < weight.shape[0])
+    return torch.where(known.unsqueeze(-1), F.embedding(torch.where(known, ids, 0), weight), nan)
 
 
 # --------------------------------------------------------------------------------------------------
