@@ -31,6 +31,8 @@ from typing import Any
 import torch
 from torch.optim.optimizer import Optimizer, ParamsT
 
+from optimizers_b200.utils import kept
+
 logger: logging.Logger = logging.getLogger(__name__)
 
 # Group keys
@@ -210,6 +212,8 @@ class GPAAdamW(Optimizer):
                 table, chunks, n_chunks = ext.build_gpa_table([(p, None, z, z, z) for p, z in zip(with_z, zs)])
                 ext.gpa_lerp(table, n_chunks, chunks, weight)
                 self.native_launches += 1
+                if kept.any_alive():
+                    kept.written(with_z)
                 mode.fill_(to_train)
                 continue
             for p in group[PARAMS]:
@@ -303,6 +307,8 @@ class GPAAdamW(Optimizer):
                 ext, (table, chunks, n_chunks) = self._table(gi, params, grads, zs, ms, vs)
                 ext.gpa_adamw_step(table, n_chunks, chunks, float(lr), beta1, beta2, eps, bc1, bc2, wd, wd_on_y, float(c), mu_y)
                 self.native_launches += 1
+                if kept.any_alive():  # (the kernel writes parameters without PyTorch's count of changes)
+                    kept.written(params)
                 continue
 
             for y, g, m, v, z in zip(params, grads, ms, vs, zs, strict=True):

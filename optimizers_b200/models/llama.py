@@ -17,6 +17,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from optimizers_b200.models import fp8, fused_ops
+from optimizers_b200.utils.kept import Kept
 
 
 @dataclass
@@ -90,7 +91,17 @@ class _Layer(nn.Module):
 
     def _fp8(self, x, out_dtype: torch.dtype, *names: str):
         held = None if torch.is_grad_enabled() else getattr(self, "_held", None)
-        return fp8.linear(x, tuple(getattr(self, n).weight if held is None else held[n] for n in names), out_dtype)
+        return fp8.linear(x, tuple(getattr(self, n).weight if held is None else self._current(n) for n in names), out_dtype)
+
+    def _current(self, name: str) -> torch.Tensor | fp8.Weight:
+        """The kept copy of a weight, or the weight itself if it has changed since."""
+        weight, kept = getattr(self, name).weight, self._held.get(name)
+        if kept is None:
+            return weight
+        if kept.of(weight):
+            return kept.value
+        del self._held[name]
+        return weight
 
     def forward_fp8(self, branch: torch.Tensor | None, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
         """The block on 8-bit products: takes and returns the last branch's output and the stream that it is still to be added to."""
@@ -129,11 +140,19 @@ class Llama(nn.Module):
                 nn.init.normal_(m.weight, mean=0.0, std=0.02)
 
     def hold_fp8_weights(self) -> None:
-        """Keep the blocks' weights in 8 bits for calls without gradients, until ``train()``; a weight that changes meanwhile needs a new call."""
+        """Keep the blocks' weights in 8 bits for calls without gradients, until ``train()``.  A weight that changes meanwhile is converted in every
+        call again, until the next call of this; changes that PyTorch does not count need that call (``utils/kept.py`` says which), and a
+        captured graph keeps what it was captured with."""
         if not self.cfg.fp8:
             raise ValueError("hold_fp8_weights needs a model with fp8=True")
+        held = []
         for layer in self.layers:
-            layer._held = {n: fp8.quantize_weight(getattr(layer, n).weight) for n in layer._LINEARS}
+            weights = {n: getattr(layer, n).weight for n in layer._LINEARS}
+            if any(type(w) not in (torch.Tensor, nn.Parameter) or w.dim() != 2 for w in weights.values()):
+                raise ValueError("hold_fp8_weights needs whole weights; shards are converted in every call")
+            held.append({n: Kept(w, fp8.quantize_weight(w)) for n, w in weights.items()})
+        for layer, kept in zip(self.layers, held):
+            layer._held = kept
 
     def train(self, mode: bool = True):
         if mode:

@@ -128,6 +128,7 @@ from optimizers_b200.preconditioner.simple import (
     SignDescentPreconditionerList,
     SpectralDescentPreconditionerList,
 )
+from optimizers_b200.utils import kept
 from optimizers_b200.utils.blocking import compress_list, split_param_groups
 from optimizers_b200.utils.state import extract_state_dict_content, update_param_state_dict_object
 
@@ -815,7 +816,12 @@ class DistributedShampoo(Optimizer):
                 self._group_step_body(rec, group, self._per_group_step)
         if self._use_cuda_streams:
             self._sync_streams_to_default()
+        self._tell_of_writes()
         return loss
+
+    def _tell_of_writes(self) -> None:
+        if kept.any_alive():  # (the native engine writes parameters without PyTorch's count of changes)
+            kept.written(p for _, group in self._groups() for p in group[PARAMS])
 
     @torch.no_grad()
     def _sync_streams_to_default(self) -> None:
@@ -848,12 +854,14 @@ class DistributedShampoo(Optimizer):
         """W ← W + (Z - W)(1 - μy): parameters become the y sequence gradients are taken at."""
         logger.info("Enabling train mode in Distributed Shampoo!")
         self._switch_mode(True)
+        self._tell_of_writes()
 
     @torch.no_grad()
     def eval(self) -> None:
         """W ← W + (Z - W)(1 - 1/μy): parameters become the averaged x sequence."""
         logger.info("Enabling eval mode in Distributed Shampoo!")
         self._switch_mode(False)
+        self._tell_of_writes()
 
     # ------------------------------------------------------------------------------------------
     # Checkpointing

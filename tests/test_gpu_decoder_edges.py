@@ -28,3 +28,47 @@ def test_tokens_outside_the_table_in_types_without_kernels(dtype):
     want[3], want[10] = 4, 2
     assert torch.equal(grad, want)
     assert fused_ops.embedding(ids, table[:0]).isnan().all()
+
+
+@pytest.mark.parametrize("optimizer", ["gpa", "gpa_mode", "shampoo", "shampoo_mode", "torch"])
+def test_weights_kept_in_8_bits_follow_steps_of_the_native_optimizers(optimizer):
+    from optimizers_b200 import AdaGradPreconditionerConfig, DistributedShampoo, GPAAdamW, GeneralizedPrimalAveragingConfig, NativeRuntimeConfig
+    from optimizers_b200.models import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig(vocab_size=300, n_layer=2, n_head=2, d_model=128, d_ffn=256, fp8=True)
+    model = Llama(cfg).cuda().eval()
+    ids = torch.arange(18, device="cuda").view(2, 9)
+
+    def step():
+        for p in model.parameters():
+            p.grad = torch.randn_like(p)
+        opt.step()
+
+    def fresh():
+        other = Llama(cfg).cuda().eval()
+        other.load_state_dict(model.state_dict())
+        return other(ids)
+
+    if optimizer.startswith("gpa"):
+        opt = GPAAdamW(model.parameters(), lr=0.01)
+    elif optimizer.startswith("shampoo"):
+        averaging = GeneralizedPrimalAveragingConfig(eval_interp_coeff=0.9, train_interp_coeff=0.7) if optimizer == "shampoo_mode" else None
+        opt = DistributedShampoo(
+            model.parameters(), lr=0.01, precondition_frequency=1, grafting_config=AdaGradPreconditionerConfig(epsilon=1e-8),
+            native_runtime_config=NativeRuntimeConfig(backend="native"), **({"iterate_averaging_config": averaging} if averaging else {}),
+        )
+    else:
+        opt = torch.optim.AdamW(model.parameters(), lr=0.01)
+    if optimizer != "torch":
+        opt.train()
+    with torch.no_grad():
+        step()
+        model.hold_fp8_weights()
+        before = model(ids)
+        assert torch.equal(before, fresh())
+        opt.eval() if optimizer.endswith("mode") else step()
+        after = model(ids)
+        assert not torch.equal(after, before) and torch.equal(after, fresh())
+        model.hold_fp8_weights()
+        assert torch.equal(model(ids), after) and all(len(layer._held) == 7 for layer in model.layers)
