@@ -279,6 +279,19 @@ def _embedding_of_known(ids: Tensor, weight: Tensor) -> Tensor:
     return torch.where(known.unsqueeze(-1), F.embedding(torch.where(known, ids, 0), weight), nan)
 
 
+class TokenEmbedding(torch.nn.Embedding):
+    """``nn.Embedding`` that looks tokens up with ``embedding`` where its caller asks for it."""
+
+    def forward(self, ids: Tensor, fused: bool = False) -> Tensor:
+        return embedding(ids, self.weight) if fused else super().forward(ids)
+
+
+def embed(module: torch.nn.Module, ids: Tensor) -> Tensor:
+    """``embedding`` through the module that holds the table, so that the module's hooks run (sharding that gathers the table, for
+    one); an ``nn.Embedding`` that was put in its place has only its table read."""
+    return embedding(ids, module.weight) if type(module) is torch.nn.Embedding else module(ids, fused=True)
+
+
 # --------------------------------------------------------------------------------------------------
 # Linear with a fast bias gradient
 # --------------------------------------------------------------------------------------------------

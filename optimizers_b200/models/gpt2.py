@@ -63,7 +63,7 @@ class GPT2(nn.Module):
     def __init__(self, cfg: GPT2Config | None = None) -> None:
         super().__init__()
         self.cfg = cfg = cfg or GPT2Config()
-        self.wte = nn.Embedding(cfg.vocab_size, cfg.d_model)
+        self.wte = fused_ops.TokenEmbedding(cfg.vocab_size, cfg.d_model)
         self.wpe = nn.Embedding(cfg.n_ctx, cfg.d_model)
         self.blocks = nn.ModuleList(_Block(cfg) for _ in range(cfg.n_layer))
         self.ln_f = nn.LayerNorm(cfg.d_model)
@@ -83,7 +83,7 @@ class GPT2(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         B, T = idx.shape
         pos = torch.arange(T, device=idx.device)
-        tokens = fused_ops.embedding(idx, self.wte.weight) if self.cfg.fused_embedding else self.wte(idx)
+        tokens = fused_ops.embed(self.wte, idx) if self.cfg.fused_embedding else self.wte(idx)
         x = tokens + self.wpe(pos)
         for blk in self.blocks:
             x = blk(x)

@@ -42,7 +42,12 @@ class RMSNorm(nn.Module):
         self.fused = fused
         self.weight = nn.Parameter(torch.ones(dim))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, branch: torch.Tensor | None = None, joined: bool = False):
+        """The norm of x, or of ``x + branch``; with ``joined`` a pair of it and the sum, in 8 bits where no gradient is wanted."""
+        if joined:
+            return _norm_of_sum(branch, x, self)
+        if branch is not None:
+            return fused_ops.add_rms_norm(branch, x, self.weight, self.eps)[0]
         if self.fused:
             return fused_ops.rms_norm(x, self.weight, self.eps)
         scale = torch.rsqrt(x.float().pow(2).mean(-1, keepdim=True) + self.eps)
@@ -75,7 +80,9 @@ class _Layer(nn.Module):
         self.w_up = nn.Linear(cfg.d_model, cfg.d_ffn, bias=False)
         self.w_down = nn.Linear(cfg.d_ffn, cfg.d_model, bias=False)
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, branch: torch.Tensor | None = None, fp8: bool = False):
+        if fp8:
+            return self.forward_fp8(branch, x, cos, sin)
         B, T, C = x.shape
         h = self.attn_norm(x)
         shape = (B, T, self.n_head, C // self.n_head)
@@ -104,15 +111,16 @@ class _Layer(nn.Module):
         return weight
 
     def forward_fp8(self, branch: torch.Tensor | None, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
-        """The block on 8-bit products: takes and returns the last branch's output and the stream that it is still to be added to."""
+        """The block on 8-bit products: takes and returns the last branch's output and the stream that it is still to be added to.  (The
+        linear layers are read, not called: several share one conversion, so hooks of theirs do not run; the block's and the norms' do.)"""
         B, T, C = x.shape
         dtype = fused_ops._compute_dtype(x)
-        h, x = _norm_of_sum(branch, x, self.attn_norm)
+        h, x = self.attn_norm(x, branch, joined=True)
         shape = (B, T, self.n_head, C // self.n_head)
         q, k, v = (t.view(shape).transpose(1, 2) for t in self._fp8(h, dtype, "wq", "wk", "wv"))
         a = F.scaled_dot_product_attention(_apply_rope(q, cos, sin), _apply_rope(k, cos, sin), v, is_causal=True)
         (branch,) = self._fp8(a.transpose(1, 2).reshape(B, T, C), dtype, "wo")
-        h, x = _norm_of_sum(branch.view(x.shape), x, self.ffn_norm)
+        h, x = self.ffn_norm(x, branch.view(x.shape), joined=True)
         gate, up = self._fp8(h, dtype, "w_gate", "w_up")
         (branch,) = self._fp8(F.silu(gate) * up, dtype, "w_down")
         return branch.view(x.shape), x
@@ -131,7 +139,7 @@ class Llama(nn.Module):
     def __init__(self, cfg: LlamaConfig | None = None) -> None:
         super().__init__()
         self.cfg = cfg = cfg or LlamaConfig()
-        self.embed = nn.Embedding(cfg.vocab_size, cfg.d_model)
+        self.embed = fused_ops.TokenEmbedding(cfg.vocab_size, cfg.d_model)
         self.layers = nn.ModuleList(_Layer(cfg) for _ in range(cfg.n_layer))
         self.norm = RMSNorm(cfg.d_model, cfg.norm_eps, cfg.fused)
         self.head = nn.Linear(cfg.d_model, cfg.vocab_size, bias=False)
@@ -163,12 +171,12 @@ class Llama(nn.Module):
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         T = idx.shape[1]
         cos, sin = _rope_tables(T, self.cfg.d_model // self.cfg.n_head, self.cfg.rope_theta, idx.device)
-        x = fused_ops.embedding(idx, self.embed.weight) if self.cfg.fused_embedding else self.embed(idx)
+        x = fused_ops.embed(self.embed, idx) if self.cfg.fused_embedding else self.embed(idx)
         if self.cfg.fp8:
             branch = None
             for layer in self.layers:
-                branch, x = layer.forward_fp8(branch, x, cos, sin)
-            h = self.norm(x) if branch is None else fused_ops.add_rms_norm(branch, x, self.norm.weight, self.norm.eps)[0]
+                branch, x = layer(x, cos, sin, branch, fp8=True)
+            h = self.norm(x) if branch is None else self.norm(x, branch)
         else:
             for layer in self.layers:
                 x = layer(x, cos, sin)

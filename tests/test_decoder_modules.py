@@ -122,3 +122,74 @@ def test_sharded_weights_are_not_kept():
         s.bind(("127.0.0.1", 0))
         port = s.getsockname()[1]
     torch.multiprocessing.spawn(_sharded_hold_worker, args=(port,), nprocs=1, join=True)
+
+
+def _small_llama(**kw):
+    torch.manual_seed(0)
+    cfg = dict(vocab_size=50, n_layer=2, n_head=2, d_model=32, d_ffn=48, fp8=True, fused_embedding=True)
+    return Llama(LlamaConfig(**(cfg | kw)))
+
+
+def test_hooks_of_blocks_norms_and_embeddings_run():
+    from optimizers_b200.models import GPT2, GPT2Config
+
+    model = _small_llama()
+    seen = []
+    watched = [model.embed, *model.layers, *(n for b in model.layers for n in (b.attn_norm, b.ffn_norm)), model.norm]
+    for m in watched:
+        m.register_forward_hook(lambda module, args, out: seen.append(module))
+    idx = torch.randint(0, 50, (2, 9))
+    model(idx[:, :-1], idx[:, 1:])
+    assert len(seen) == len(watched) and all(any(m is s for s in seen) for m in watched)
+    seen.clear()
+    with torch.no_grad():
+        model(idx)
+    assert len(seen) == len(watched)
+    gpt = GPT2(GPT2Config(vocab_size=50, n_ctx=16, n_layer=1, n_head=2, d_model=32, d_mlp=48, fused_embedding=True))
+    seen.clear()
+    gpt.wte.register_forward_hook(lambda module, args, out: seen.append(module))
+    gpt(idx)
+    assert seen == [gpt.wte]
+
+
+def test_an_embedding_put_in_place_of_the_models_is_read():
+    model = _small_llama()
+    idx = torch.randint(0, 50, (2, 9))
+    want = model(idx)
+    table = model.embed.weight.detach().clone()
+    model.embed = torch.nn.Embedding(50, 32, _weight=table)
+    assert torch.equal(model(idx), want)
+
+
+def _sharded_worker(rank, port):
+    import torch.distributed as dist
+    from torch.distributed.fsdp import fully_shard
+
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2)
+    idx = torch.randint(0, 50, (2, 9), generator=torch.Generator().manual_seed(1))
+    whole = _small_llama()
+    loss = whole(idx[:, :-1], idx[:, 1:])
+    loss.backward()
+    model = _small_llama()
+    for part in (model.embed, *model.layers, model.norm):
+        fully_shard(part)
+    fully_shard(model)
+    got = model(idx[:, :-1], idx[:, 1:])
+    got.backward()
+    assert torch.equal(got, loss)
+    for (name, p), q in zip(model.named_parameters(), whole.parameters()):
+        assert torch.allclose(p.grad.full_tensor(), q.grad, rtol=1e-6, atol=1e-9), name  # the mean of two equal gradients
+    model.eval()
+    whole.eval()
+    with torch.no_grad():
+        assert torch.equal(model(idx), whole(idx))
+    dist.destroy_process_group()
+
+
+def test_blocks_norm_and_embedding_sharded_on_their_own():
+    import socket
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    torch.multiprocessing.spawn(_sharded_worker, args=(port,), nprocs=2, join=True)
