@@ -88,6 +88,54 @@ def _dense(g: Tensor) -> bool:
     return True
 
 
+def _share_a_value(a: Tensor, b: Tensor) -> bool:
+    """Whether some byte belongs to an element of each.  An element of ``a`` and one of ``b`` meet where the distance of the two starts is a sum of
+    strides times differences of indices (a byte within an element counts as a last dimension of stride one): looked for from the
+    largest stride down, among the multiples that the smaller strides can still make up for."""
+    reach: dict[int, list[int]] = {}  # stride in bytes -> least and greatest multiple
+    for t, low in ((a, False), (b, True)):
+        size = t.element_size()
+        for n, st in [*((n, st * size) for n, st in zip(t.shape, t.stride())), (size, 1)]:
+            span = reach.setdefault(st, [0, 0])
+            span[0 if low else 1] += (1 - n) if low else (n - 1)
+    steps = [(st, lo, hi) for st, (lo, hi) in sorted(reach.items(), reverse=True) if st > 0 and lo < hi]
+    below = [(0, 0)]  # what the steps behind each one can add up to
+    for st, lo, hi in reversed(steps):
+        below.append((below[-1][0] + st * lo, below[-1][1] + st * hi))
+    below.reverse()
+    tries = 100_000  # (layouts that take more do not come up; they count as shared)
+    work = [(0, b.data_ptr() - a.data_ptr())]
+    while work and tries > 0:
+        k, left = work.pop()
+        tries -= 1
+        if k == len(steps):
+            if left == 0:
+                return True
+            continue
+        st, lo, hi = steps[k]
+        least, most = below[k + 1]
+        first, last = max(lo, -((most - left) // st)), min(hi, (left - least) // st)
+        work.extend((k + 1, left - st * t) for t in range(first, min(last, first + tries) + 1))
+    return bool(work)
+
+
+def _check_disjoint(grads: list[Tensor]) -> None:
+    """Raise ``ValueError`` for two gradients that share memory."""
+    spans = []
+    for g in grads:
+        if type(g) is Tensor and g.numel() > 0 and g.device.type != "meta":
+            reach = sum((n - 1) * st for n, st in zip(g.shape, g.stride())) + 1
+            spans.append((str(g.device), g.data_ptr(), g.data_ptr() + reach * g.element_size(), g))
+    spans.sort(key=lambda span: span[:3])
+    open_spans: list = []
+    for device, start, end, g in spans:
+        open_spans = [o for o in open_spans if o[0] == device and o[2] > start]
+        for o in open_spans:
+            if _share_a_value(o[3], g):
+                raise ValueError("clip: two gradients share memory; each value can be scaled once only")
+        open_spans.append((device, start, end, g))
+
+
 def _packed(grads: list[Tensor]) -> list[Tensor]:
     """The gradients, with copies in place of those that leave gaps in their memory."""
     return [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
@@ -153,6 +201,8 @@ def clip_grad_norm_(
             raise ValueError("a gradient with an expanded dimension cannot be scaled in place")
     native = _native(grads)
     work = _packed(grads) if native else grads
+    if not native or any(w is not g for w, g in zip(work, grads)):  # (the kernels' entry looks at what it is given, which are copies then)
+        _check_disjoint(grads)
     sumsq = _sumsq(work, shard_group, native, disjoint=True)
     if error_if_nonfinite:
         value = float(sumsq.sum().sqrt())
