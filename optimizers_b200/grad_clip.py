@@ -21,6 +21,14 @@ import torch.distributed as dist
 from torch import Tensor
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_on_sm100: dict[int | None, bool] = {}
+
+
+def _sm100(device: torch.device) -> bool:
+    known = _on_sm100.get(device.index)
+    if known is None:
+        known = _on_sm100[device.index] = torch.cuda.get_device_capability(device)[0] == 10
+    return known
 
 
 def _gradients(parameters: Tensor | Iterable[Tensor], shard_group) -> list[Tensor]:
@@ -62,7 +70,7 @@ def _native(grads: list[Tensor]) -> bool:
     return (
         d.type == "cuda"
         and all(type(g) is Tensor and g.device == d and g.dtype in _FLOATS for g in grads)
-        and torch.cuda.get_device_capability(d)[0] == 10
+        and _sm100(d)
     )
 
 
@@ -187,7 +195,7 @@ def clip_grad_norm_(
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f"Invalid max_norm: {max_norm}")
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
-    if shard_group is None and not error_if_nonfinite and parameters and getattr(parameters[0], "is_cuda", False):
+    if shard_group is None and not error_if_nonfinite and parameters and getattr(parameters[0], "is_cuda", False) and _sm100(parameters[0].device):
         from optimizers_b200.ops import build
 
         norm = build.load().clip_parameters(parameters, max_norm)

@@ -78,3 +78,26 @@ def _indices(shape):
     import itertools
 
     return itertools.product(*(range(n) for n in shape))
+
+
+class _OnAnotherGpu(torch.nn.Parameter):
+    """A parameter that takes itself for one on a GPU without these kernels."""
+
+    is_cuda = True
+
+
+def test_other_gpus_do_without_the_extension(monkeypatch):
+    from optimizers_b200 import grad_clip
+    from optimizers_b200.ops import build
+
+    def load():
+        raise AssertionError("the extension was loaded")
+
+    monkeypatch.setattr(build, "load", load)
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda device=None: (9, 0))
+    monkeypatch.setattr(grad_clip, "_on_sm100", {}, raising=False)
+    p = _OnAnotherGpu(torch.zeros(5))
+    p.grad = torch.full((5,), 3.0)
+    assert float(clip_grad_norm_([p], 1.0)) == pytest.approx(math.sqrt(45), rel=1e-6)
+    assert p.grad.norm() == pytest.approx(1.0, rel=1e-5)
+    assert float(grad_norm(p)) == pytest.approx(1.0, rel=1e-5)
