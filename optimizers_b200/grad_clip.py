@@ -75,9 +75,9 @@ def _native(grads: list[Tensor]) -> bool:
 
 
 def _sum_over_group(sumsq: Tensor, shard_group) -> Tensor:
-    total = sumsq.sum().reshape(1)
+    total = sumsq.sum().reshape(1).double()  # one type on every rank, whatever gradients it holds
     dist.all_reduce(total, group=shard_group)
-    return total
+    return total.to(sumsq.dtype)
 
 
 def _plain_sumsq(grads: list[Tensor]) -> Tensor:
@@ -150,10 +150,18 @@ def _packed(grads: list[Tensor]) -> list[Tensor]:
 
 
 def _no_gradients(parameters, shard_group) -> Tensor:
-    """The norm where this rank holds no gradient (others may)."""
-    device = next((p.device for p in ([parameters] if isinstance(parameters, Tensor) else parameters)), torch.device("cpu"))
+    """The sum of squares where this rank holds no gradient (others may)."""
+    device = next((p.device for p in ([parameters] if isinstance(parameters, Tensor) else parameters)), None)
+    if device is None:
+        device = torch.device("cuda" if shard_group is not None and dist.get_backend(shard_group) == "nccl" else "cpu")
     zero = torch.zeros(1, device=device)
-    return (_sum_over_group(zero, shard_group) if shard_group is not None else zero).sqrt()[0]
+    return _sum_over_group(zero, shard_group) if shard_group is not None else zero
+
+
+def _refuse_nonfinite(sumsq: Tensor) -> None:
+    value = float(sumsq.sum().sqrt())
+    if not math.isfinite(value):
+        raise RuntimeError(f"The norm of the gradients is {value}, so they cannot be clipped")
 
 
 @torch.no_grad()
@@ -162,7 +170,7 @@ def grad_norm(parameters: Tensor | Iterable[Tensor], *, shard_group: dist.Proces
     parameters = parameters if isinstance(parameters, Tensor) else list(parameters)
     grads = _gradients(parameters, shard_group)
     if not grads:
-        return _no_gradients(parameters, shard_group)
+        return _no_gradients(parameters, shard_group).sqrt()[0]
     native = _native(grads)
     return _sumsq(_packed(grads) if native else grads, shard_group, native, disjoint=False).sum().sqrt()
 
@@ -203,7 +211,10 @@ def clip_grad_norm_(
             return norm
     grads = _gradients(parameters, shard_group)
     if not grads:
-        return _no_gradients(parameters, shard_group)
+        sumsq = _no_gradients(parameters, shard_group)
+        if error_if_nonfinite:  # on every rank of the group or on none
+            _refuse_nonfinite(sumsq)
+        return sumsq.sqrt()[0]
     for g in grads:
         if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
             raise ValueError("a gradient with an expanded dimension cannot be scaled in place")
@@ -213,9 +224,7 @@ def clip_grad_norm_(
         _check_disjoint(grads)
     sumsq = _sumsq(work, shard_group, native, disjoint=True)
     if error_if_nonfinite:
-        value = float(sumsq.sum().sqrt())
-        if not math.isfinite(value):
-            raise RuntimeError(f"The norm of the gradients is {value}, so they cannot be clipped")
+        _refuse_nonfinite(sumsq)
     if native:
         from optimizers_b200.ops import build
 

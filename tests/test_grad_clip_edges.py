@@ -101,3 +101,33 @@ def test_other_gpus_do_without_the_extension(monkeypatch):
     assert float(clip_grad_norm_([p], 1.0)) == pytest.approx(math.sqrt(45), rel=1e-6)
     assert p.grad.norm() == pytest.approx(1.0, rel=1e-5)
     assert float(grad_norm(p)) == pytest.approx(1.0, rel=1e-5)
+
+
+def _uneven_worker(rank, port):
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2)
+    p = torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))
+    if rank == 0:
+        p.grad = torch.full((4,), 3.0, dtype=torch.float64)
+    # gradients of other types on other ranks, or none
+    assert abs(float(clip_grad_norm_([p], 12.0, shard_group=dist.group.WORLD)) - 6.0) < 1e-6
+    assert abs(float(grad_norm([p] if rank == 0 else [], shard_group=dist.group.WORLD)) - 6.0) < 1e-6
+    if rank == 1:
+        p = torch.nn.Parameter(torch.zeros(4))
+        p.grad = torch.full((4,), 4.0)
+    assert abs(float(grad_norm([p], shard_group=dist.group.WORLD)) - 10.0) < 1e-6
+    # a norm that is refused is refused on every rank
+    q = torch.nn.Parameter(torch.zeros(2))
+    if rank == 0:
+        q.grad = torch.tensor([1.0, math.inf])
+    with pytest.raises(RuntimeError, match="norm of the gradients"):
+        clip_grad_norm_([q], 1.0, shard_group=dist.group.WORLD, error_if_nonfinite=True)
+    dist.destroy_process_group()
+
+
+def test_ranks_with_other_gradients_or_none_agree():
+    import socket
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.spawn(_uneven_worker, args=(port,), nprocs=2, join=True)
