@@ -26,6 +26,7 @@ from dataclasses import dataclass
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from optimizers_b200.models import fused_ops
@@ -172,6 +173,11 @@ def _is_native(x: Tensor) -> bool:
     return fused_ops._kernels_take(x) and x.numel() > 0
 
 
+def _has_tangent(*tensors: Tensor) -> bool:
+    """Whether a forward-mode derivative is being taken along one of these."""
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _rows_of(data: Tensor, scale: Tensor) -> Rows:
     """Rows without the checks, for results of the kernels."""
     rows = object.__new__(Rows)
@@ -218,6 +224,8 @@ def add_rms_norm(x: Tensor, residual: Tensor | None, weight: Tensor, eps: float 
     fused_ops._check_add_norm(x, residual, weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         raise ValueError("8-bit rows carry no gradient; use fused_ops.add_rms_norm in training, or torch.no_grad()")
+    if _has_tangent(*(t for t in (x, residual, weight) if t is not None)):
+        raise ValueError("8-bit rows carry no forward-mode derivative; use fused_ops.add_rms_norm")
     return _norm_rows(x, residual, weight, eps)
 
 
@@ -255,6 +263,7 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
 
     ``out_dtype``: fp32 or bf16; by default the autocast dtype, or x's (bf16 for ``Rows``).  Gradients flow to ``x`` and to weights that
     are tensors; a ``Weight`` or ``Rows`` takes no gradient, and combining one with an operand that needs one raises ``ValueError``.
+    Forward-mode derivatives raise ``ValueError`` too.
     """
     several = not isinstance(weight, (Tensor, Weight))
     weights = tuple(weight) if several else (weight,)
@@ -284,6 +293,8 @@ def linear(x: Tensor | Rows, weight: Tensor | Weight | Sequence[Tensor | Weight]
     learns = torch.is_grad_enabled() and any(t.requires_grad for t in operands)
     if learns and (held_x or len(tensors) < len(weights)):
         raise ValueError("operands held in 8 bits carry no gradient: pass tensors for x and every weight in training, or use torch.no_grad()")
+    if _has_tangent(*operands):
+        raise ValueError("linear has no forward-mode derivative: its operands are rounded to 8 bits")
     if native and not held_x and len(tensors) == len(weights):
         out = fused_ops._ext().fp8_linear(x, tensors, out_dtype == torch.bfloat16, _status_of(x.device))
     elif native and not held_x and not tensors:

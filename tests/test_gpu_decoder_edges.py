@@ -72,3 +72,20 @@ def test_weights_kept_in_8_bits_follow_steps_of_the_native_optimizers(optimizer)
         assert not torch.equal(after, before) and torch.equal(after, fresh())
         model.hold_fp8_weights()
         assert torch.equal(model(ids), after) and all(len(layer._held) == 7 for layer in model.layers)
+
+
+def test_forward_mode_derivatives_are_refused():
+    x, w, t = _x(4, 144, F32), _x(6, 144, F32, 1), _x(4, 144, F32, 2)
+    held, ones, table, ids = fp8.quantize_weight(w), torch.ones(144, device="cuda"), _x(30, 144, F32, 3), torch.arange(4, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, t)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: fp8.linear(dual, w), lambda: fp8.linear(dual, held), lambda: fp8.linear(x, dual), lambda: fp8.add_rms_norm(dual, x, ones)):
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        call()
+                for call in (lambda: fused_ops.add_rms_norm(dual, x, ones), lambda: fused_ops.add_rms_norm(x, dual, ones), lambda: fused_ops.embedding(ids, dual)):
+                    with pytest.raises((RuntimeError, NotImplementedError)):
+                        call()
+        fp8.linear(x, w)
+        fused_ops.embedding(ids, table)
