@@ -212,7 +212,7 @@ def _norm_rows(x: Tensor, residual: Tensor | None, weight: Tensor, eps: float) -
         )
         fused_ops._count()
         return _rows_of(_e4m3(raw, C), scale.t()), (x if residual is None else h)
-    h = x if residual is None else (x.float() + residual.float()).to(torch.promote_types(x.dtype, residual.dtype))
+    h = x if residual is None else fused_ops._sum_of(x, residual)
     hf = h.float().reshape(-1, C)
     y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
     return Rows(*_plain_groups(y, 1)), h

@@ -241,10 +241,20 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6)
     out_dtype = _norm_out_dtype(x)
     if _kernels_take(x, residual, weight) and 0 < x.shape[-1] <= _MOST_COLUMNS and x.numel() > 0:
         return _ext().add_rms_norm(x, residual, weight, eps, out_dtype == torch.bfloat16)
-    h = (x.float() + residual.float()).to(torch.promote_types(x.dtype, residual.dtype))
-    hf = h.float()
+    h = _sum_of(x, residual)
+    hf = _at_least_32_bits(h)
     y = hf * torch.rsqrt(hf.pow(2).mean(-1, keepdim=True) + eps)
-    return (y * weight.float()).to(out_dtype), h
+    return (y * weight.to(hf.dtype)).to(out_dtype), h
+
+
+def _at_least_32_bits(x: Tensor) -> Tensor:
+    return x.to(torch.promote_types(x.dtype, torch.float32))
+
+
+def _sum_of(x: Tensor, residual: Tensor) -> Tensor:
+    """The sum in the wider of the two types, rounded once."""
+    h = _at_least_32_bits(x) + _at_least_32_bits(residual)
+    return h.to(torch.promote_types(x.dtype, residual.dtype))
 
 
 # --------------------------------------------------------------------------------------------------
@@ -267,7 +277,7 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.
     if _kernels_take(weight) and type(ids) is torch.Tensor and ids.device == weight.device and out_dtype in _KINDS and weight.numel() > 0:
         return _ext().embedding(ids, weight, scale, out_dtype == torch.bfloat16)
     y = F.embedding(ids, weight) if ids.device.type == "cpu" else _embedding_of_known(ids, weight)
-    return y.to(out_dtype) if scale == 1.0 else (y.float() * scale).to(out_dtype)
+    return y.to(out_dtype) if scale == 1.0 else (_at_least_32_bits(y) * scale).to(out_dtype)
 
 
 def _embedding_of_known(ids: Tensor, weight: Tensor) -> Tensor:

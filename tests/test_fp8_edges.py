@@ -24,3 +24,15 @@ def test_forward_mode_derivatives_are_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
                     call(dual)
             call(x.clone())  # the level alone changes nothing
+
+
+def test_fp64_is_computed_in_64_bits():
+    torch.manual_seed(0)
+    x, r, w = (torch.randn(5, 48, dtype=F64), torch.randn(5, 48, dtype=F64), torch.randn(48, dtype=F64))
+    y, h = fused_ops.add_rms_norm(x, r, w, eps=1e-5)
+    assert y.dtype == h.dtype == F64 and torch.equal(h, x + r)
+    want = h * (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * w
+    assert ((y - want).abs() <= 60 * 2**-53 * want.abs()).all()  # a mean of 48 squares, its root, two products
+    assert torch.equal(fp8.add_rms_norm(x, r, w)[1], h) and torch.equal(fused_ops.add_rms_norm(x.float(), r, w)[1], x.float().double() + r)
+    table, ids = torch.randn(11, 6, dtype=F64), torch.randint(0, 11, (20,))
+    assert torch.equal(fused_ops.embedding(ids, table, scale=1 / 3), table[ids] * (1 / 3))
