@@ -175,6 +175,8 @@ def _is_native(x: Tensor) -> bool:
 
 def _has_tangent(*tensors: Tensor) -> bool:
     """Whether a forward-mode derivative is being taken along one of these."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # none is being taken (the look below costs a microsecond a tensor)
+        return False
     return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
