@@ -99,7 +99,8 @@ def _status_of(device: torch.device) -> Tensor:
     if status is None:
         if torch.cuda.is_current_stream_capturing():  # it would live in that graph's memory
             raise RuntimeError("call fp8.linear once on this device before capturing it into a CUDA graph")
-        status = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # it serves the calls of every mode
+            status = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
     return status
 
 

@@ -133,7 +133,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       launches += 2;
     }
     ++launches;
-    saved.push_back(status);
+    ctx->saved_data["status"] = status;  // a word of its own, no operand: whatever mode it was made in
     ctx->save_for_backward(std::move(saved));
     ctx->saved_data["learns"] = learns;
     ctx->saved_data["types"] = types;
@@ -151,7 +151,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     const bool need_dx = learns & 1, need_dw = learns >> 1;
     const auto types = ctx->saved_data["types"].toIntVector();
     const auto shape = ctx->saved_data["shape"].toIntVector();
-    const Tensor& status = saved.back();
+    const Tensor status = ctx->saved_data["status"].toTensor();
     const size_t first = need_dw ? 2 : 0, n = types.size();
     size_t last = 0;
     for (size_t i = 0; i < n; ++i)

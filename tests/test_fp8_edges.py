@@ -36,3 +36,16 @@ def test_fp64_is_computed_in_64_bits():
     assert torch.equal(fp8.add_rms_norm(x, r, w)[1], h) and torch.equal(fused_ops.add_rms_norm(x.float(), r, w)[1], x.float().double() + r)
     table, ids = torch.randn(11, 6, dtype=F64), torch.randint(0, 11, (20,))
     assert torch.equal(fused_ops.embedding(ids, table, scale=1 / 3), table[ids] * (1 / 3))
+
+
+def test_status_words_made_in_inference_mode_serve_every_mode(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(fp8, "_status", {})
+    with torch.inference_mode():
+        status = fp8._status_of(torch.device("cpu"))
+    assert not status.is_inference() and fp8._status_of(torch.device("cpu")) is status
+    fp8.check_status()
+    status.fill_(1)
+    with pytest.raises(RuntimeError, match="gave up a wait"):
+        fp8.check_status()
+    fp8.check_status()

@@ -89,3 +89,15 @@ def test_forward_mode_derivatives_are_refused():
                         call()
         fp8.linear(x, w)
         fused_ops.embedding(ids, table)
+
+
+def test_first_product_in_inference_mode_then_training(monkeypatch):
+    monkeypatch.setattr(fp8, "_status", {})
+    x, w = _x(20, 256), _x(64, 256, F32, 1)
+    with torch.inference_mode():
+        want = fp8.linear(x, w).clone()
+    got = fp8.linear(x.requires_grad_(), w.requires_grad_())
+    assert torch.equal(got, want)
+    got.sum().backward()
+    assert x.grad.isfinite().all() and w.grad.isfinite().all()
+    fp8.check_status()
