@@ -119,14 +119,15 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     if (need_dw) std::tie(q, s, qt, st) = fp8_both(x2);
     else std::tie(q, s) = fp8_rows(x2);
     variable_list saved, out;
-    if (need_dw) saved = {bytes(qt, T), st.t()};
+    // Operands are kept whole, with their padding: hooks on saved tensors may copy them, and a copy of a slice would lose its pitch.
+    if (need_dw) saved = {qt, st.t()};
     std::vector<int64_t> sizes = x.sizes().vec(), shapes, types;
     for (const Tensor& w : weights) {
       auto [qw, qwt, sw] = fp8_squares(w.contiguous(), need_dx);
       sizes.back() = w.size(0);
       out.push_back(fp8_matmul(bytes(q, K), s.t(), bytes(qw, K), sw, false, out_bf16, std::nullopt, status, sizes));
       if (need_dx) {
-        saved.push_back(bytes(qwt, w.size(0)));
+        saved.push_back(qwt);
         saved.push_back(sw.t());
       }
       types.push_back(is_bf16(w));
@@ -171,11 +172,11 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       ++launches;
       if (need_dx) {  // sums over several layers stay in 32 bits until the last
         const bool bf16 = i == last && ctx->saved_data["x_bf16"].toBool();
-        dx = fp8_matmul(bytes(q, N), s.t(), saved[first + 2 * i], saved[first + 2 * i + 1], false, bf16, dx.defined() ? std::optional<Tensor>(dx) : std::nullopt, status, shape);
+        dx = fp8_matmul(bytes(q, N), s.t(), bytes(saved[first + 2 * i], N), saved[first + 2 * i + 1], false, bf16, dx.defined() ? std::optional<Tensor>(dx) : std::nullopt, status, shape);
         ++launches;
       }
       if (want_dw) {
-        out[1 + i] = fp8_matmul(bytes(qt, T), st.t(), saved[0], saved[1], true, types[i], std::nullopt, status, std::nullopt);
+        out[1 + i] = fp8_matmul(bytes(qt, T), st.t(), bytes(saved[0], T), saved[1], true, types[i], std::nullopt, status, std::nullopt);
         ++launches;
       }
     }

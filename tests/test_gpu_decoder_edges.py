@@ -101,3 +101,23 @@ def test_first_product_in_inference_mode_then_training(monkeypatch):
     got.sum().backward()
     assert x.grad.isfinite().all() and w.grad.isfinite().all()
     fp8.check_status()
+
+
+@pytest.mark.parametrize("size", [(1001, 333, 1337), (5, 33, 200), (64, 128, 256)])
+def test_saved_tensors_that_hooks_copy(size):
+    """Operands saved for the backward pass come back from a copy: on the host, or packed by a hook of the caller's."""
+    T, N, K = size
+    x, ws, r = _x(T, K).requires_grad_(), [_x(n, K, F32, n).requires_grad_() for n in (N, N + 3)], _x(T, K, F32, 2).requires_grad_()
+    norm = (torch.rand(K, device="cuda") + 0.5).requires_grad_()
+    dys = [_x(T, n, BF16, n + 1) for n in (N, N + 3)]
+
+    def call():
+        h, _ = fused_ops.add_rms_norm(x, r, norm)
+        return torch.autograd.grad(fp8.linear(h, tuple(ws)), [x, r, norm, *ws], dys)
+
+    want = call()
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t)):
+        with hooks:
+            got = call()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
