@@ -27,7 +27,6 @@ from dataclasses import dataclass
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from optimizers_b200.models import fused_ops
 
@@ -232,6 +231,18 @@ def add_rms_norm(x: Tensor, residual: Tensor | None, weight: Tensor, eps: float 
     return _norm_rows(x, residual, weight, eps)
 
 
+class _Once(torch.autograd.Function):
+    """A gradient that raises an error where somebody differentiates it again."""
+
+    @staticmethod
+    def forward(ctx, grad: Tensor):  # type: ignore[override]
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad: Tensor):  # type: ignore[override]
+        raise RuntimeError("this operator's gradient cannot be differentiated again")
+
+
 class _Linear(torch.autograd.Function):
     """The plain form of the layer; the kernels' is a node of the extension."""
 
@@ -245,8 +256,16 @@ class _Linear(torch.autograd.Function):
         return tuple(_plain_product(rows, sq, GROUP, dtype) for sq in squares)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):  # type: ignore[override]
+        learns = ctx.needs_input_grad
+        # dx depends on the weights and dW on x, whether or not what comes in depends on a leaf
+        again = torch.is_grad_enabled() and ((learns[0] and any(learns[2:])) or any(dy is not None and dy.requires_grad for dy in grads))
+        with torch.no_grad():
+            out = _Linear._gradients(ctx, grads)
+        return tuple(None if g is None else _Once.apply(g.detach().requires_grad_()) if again else g for g in out)
+
+    @staticmethod
+    def _gradients(ctx, grads):
         x_dtype, w_dtypes = ctx.meta
         saved = ctx.saved_tensors
         dx, dws = None, [None] * len(w_dtypes)

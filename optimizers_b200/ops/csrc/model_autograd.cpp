@@ -37,10 +37,11 @@ Tensor readable(const Tensor& t) {
   return (t.scalar_type() == torch::kFloat32 || is_bf16(t) ? t : t.to(torch::kFloat32)).contiguous();
 }
 
-// Gradients that raise an error where somebody differentiates them again.
-variable_list once(const variable_list& incoming, variable_list out, bool recorded) {
+// Gradients that raise an error where somebody differentiates them again: they depend on a leaf through what comes in or, `depends`, through what
+// the node itself keeps.
+variable_list once(const variable_list& incoming, variable_list out, bool recorded, bool depends) {
   if (!recorded) return out;
-  bool any = false;
+  bool any = depends;
   for (const auto& g : incoming) any = any || (g.defined() && g.requires_grad());
   if (!any) return out;
   torch::AutoGradMode on(true);
@@ -75,11 +76,11 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
     const Tensor &dy = grads[0], &dh = grads[1];
     if (!dy.defined()) {  // only the sum was used
       if (!dh.defined()) return variable_list(5);
-      return once(grads, {dh.to(x_type, false, true), dh.to(r_type, false, true), torch::zeros_like(w), Tensor(), Tensor()}, recorded);
+      return once(grads, {dh.to(x_type, false, true), dh.to(r_type, false, true), torch::zeros_like(w), Tensor(), Tensor()}, recorded, false);
     }
     auto [dx, dr, dw] = add_norm_bwd(readable(dy), dh.defined() ? std::optional<Tensor>(dh.to(h.scalar_type()).contiguous()) : std::nullopt, h, w, rstd, x_bf16, true);
     launches += 2;
-    return once(grads, {dx, dr.scalar_type() == r_type ? dr : dr.to(r_type), dw, Tensor(), Tensor()}, recorded);
+    return once(grads, {dx, dr.scalar_type() == r_type ? dr : dr.to(r_type), dw, Tensor(), Tensor()}, recorded, true);
   }
 };
 
@@ -100,7 +101,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const Tensor ids = ctx->get_saved_variables()[0];
     launches += 3;
     Tensor dw = embed_bwd(ids, readable(grads[0]), ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["bf16"].toBool());
-    return once(grads, {Tensor(), dw, Tensor(), Tensor()}, recorded);
+    return once(grads, {Tensor(), dw, Tensor(), Tensor()}, recorded, false);
   }
 };
 
@@ -181,7 +182,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       }
     }
     out[0] = dx;
-    return once(grads, std::move(out), recorded);
+    return once(grads, std::move(out), recorded, need_dx && need_dw);
   }
 };
 

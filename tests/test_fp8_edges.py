@@ -49,3 +49,18 @@ def test_status_words_made_in_inference_mode_serve_every_mode(monkeypatch):
     with pytest.raises(RuntimeError, match="gave up a wait"):
         fp8.check_status()
     fp8.check_status()
+
+
+def test_second_derivatives_are_never_lost_silently():
+    """dx depends on the weight and dW on x, also where what comes in is a constant: a sum of a gradient with other terms has to raise."""
+    x, w = torch.randn(4, 130, requires_grad=True), torch.randn(6, 130, requires_grad=True)
+    for leaf, other in ((x, w), (w, x)):
+        (g,) = torch.autograd.grad(fp8.linear(x, w).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="again"):
+            (g.square().sum() + other.sum()).backward()
+    # where only one side learns its gradient is a constant
+    (g,) = torch.autograd.grad(fp8.linear(x, w.detach()).sum(), x, create_graph=True)
+    assert not g.requires_grad
+    (g,) = torch.autograd.grad(fp8.linear(x, w.detach()).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="again"):
+        g.sum().backward()

@@ -121,3 +121,17 @@ def test_saved_tensors_that_hooks_copy(size):
             got = call()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_never_lost_silently():
+    """Gradients depend on the operands also where what comes in is a constant: a sum of a gradient with other terms has to raise."""
+    x, w = _x(9, 130, F32).requires_grad_(), _x(20, 130, F32, 1).requires_grad_()
+    r, n, table = _x(9, 130, F32, 2).requires_grad_(), torch.ones(130, device="cuda", requires_grad=True), _x(30, 16, F32).requires_grad_()
+    ids = torch.arange(4, device="cuda")
+    for out, leaf in ((fp8.linear(x, w), x), (fp8.linear(x, w), w), (fused_ops.add_rms_norm(x, r, n)[0], x)):
+        (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="again"):
+            (g.square().sum() + w.sum()).backward()
+    for out, leaf in ((fp8.linear(x, w.detach()), x), (fused_ops.embedding(ids, table), table), (fused_ops.add_rms_norm(x, r, n)[1], x)):
+        (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        assert not g.requires_grad  # a constant
