@@ -785,6 +785,36 @@ torch::Tensor bytes_of(const torch::Tensor& like, int64_t rows, int64_t cols) {
   return torch::empty({rows, up16(cols)}, like.options().dtype(torch::kUInt8));
 }
 
+struct ProductPlan {
+  int n;  // columns of a tile; 256, and uncut 128 with a scale per row of B, by pairs of CTAs
+  int splits;
+};
+
+// The shape of a tile by what the product would take with it: waves of tiles times the time of one group step of a tile, in units of a step of 128 x 128
+// (measured on 16384 x 8192 x 2048: 269 us with pairs, 326 with 128 x 128, 644 with 128 x 64; a scale per row of B: 482, 499 as pairs of 256 x 128,
+// 695).  Tiles of single CTAs are cut along K among up to eight while SMs are idle; joining two or
+// four takes about two steps, eight (which have to start on one GPC) about twelve.
+ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool column, int sms) {
+  auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+  const int64_t groups = groups_of(K);
+  const double wide_step = column ? 1.93 : 1.63, narrow_step = column ? 0.7 : 1.0;
+  const double wide = up(up(M, 256) * up(N, 256), sms / 2) * wide_step * groups;
+  const double middle = (column ? up(up(M, 256) * up(N, 128), sms / 2) : up(up(M, 128) * up(N, 128), sms)) * static_cast<double>(groups);
+  double best = std::min(wide, middle);
+  ProductPlan plan{wide <= middle ? 256 : 128, 1};
+  for (int n : {64, 128}) {
+    const int64_t tiles = up(M, 128) * up(N, n);
+    for (int s = n == 64 ? 1 : 2; s <= kMaxSplits && (s == 1 || (tiles * s <= sms && groups >= 2 * s)); s *= 2) {
+      const double t = up(tiles * s, sms) * (n == 64 ? narrow_step : 1.) * up(groups, s) + (s == 8 ? 12. : s > 1 ? 2. : 0.);
+      if (t < best) {
+        best = t;
+        plan = {n, s};
+      }
+    }
+  }
+  return plan;
+}
+
 void check_operand(const torch::Tensor& a, const torch::Tensor& s, const char* what) {
   TORCH_CHECK(a.is_cuda() && a.dim() == 2 && a.scalar_type() == torch::kUInt8, "fp8: operand ", what, " is a CUDA matrix of e4m3 bytes");
   TORCH_CHECK(a.stride(1) == 1 && a.stride(0) % 16 == 0 && a.stride(0) >= a.size(1) && reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0,
@@ -906,32 +936,12 @@ torch::Tensor fp8_matmul(const torch::Tensor& a, const torch::Tensor& sa, const 
     cfg.numAttrs = per_tile > 1 ? 1 : 0;
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_c, p));
   };
-  // The shape of a tile by what the product would take with it: waves of tiles times the time of one group step of a tile, in units of a step of 128 x 128
-  // (measured on 16384 x 8192 x 2048: 269 us with pairs, 326 with 128 x 128, 644 with 128 x 64; a scale per row of B: 482, 499 as pairs of 256 x 128,
-  // 695).  Tiles of single CTAs are cut along K among up to eight while SMs are idle; joining two or
-  // four takes about two steps, eight (which have to start on one GPC) about twelve.
   auto with_n = [&](auto column, auto out_tag) {
     constexpr bool kColumn = decltype(column)::value;
-    auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
-    const double wide_step = kColumn ? 1.93 : 1.63, narrow_step = kColumn ? 0.7 : 1.0;
-    const double wide = up(up(M, 256) * up(N, 256), sms / 2) * wide_step * p.groups;
-    const double middle = (kColumn ? up(up(M, 256) * up(N, 128), sms / 2) : up(up(M, 128) * up(N, 128), sms)) * static_cast<double>(p.groups);
-    double best = std::min(wide, middle);
-    int cut_n = 0, splits = 1;
-    for (int n : {64, 128}) {
-      const int64_t tiles = up(M, 128) * up(N, n);
-      for (int s = n == 64 ? 1 : 2; s <= kMaxSplits && (s == 1 || (tiles * s <= sms && p.groups >= 2 * s)); s *= 2) {
-        const double t = up(tiles * s, sms) * (n == 64 ? narrow_step : 1.) * up(p.groups, s) + (s == 8 ? 12. : s > 1 ? 2. : 0.);
-        if (t < best) {
-          best = t;
-          cut_n = n;
-          splits = s;
-        }
-      }
-    }
-    if (cut_n == 64) go(std::integral_constant<int, 64>{}, std::false_type{}, column, out_tag, splits);
-    else if (cut_n == 128) go(std::integral_constant<int, 128>{}, std::false_type{}, column, out_tag, splits);
-    else if (wide <= middle) go(std::integral_constant<int, 256>{}, std::true_type{}, column, out_tag, 1);
+    const ProductPlan plan = plan_product(M, N, K, kColumn, sms);
+    if (plan.n == 64) go(std::integral_constant<int, 64>{}, std::false_type{}, column, out_tag, plan.splits);
+    else if (plan.n == 256) go(std::integral_constant<int, 256>{}, std::true_type{}, column, out_tag, 1);
+    else if (plan.splits > 1) go(std::integral_constant<int, 128>{}, std::false_type{}, column, out_tag, plan.splits);
     else go(std::integral_constant<int, 128>{}, std::integral_constant<bool, kColumn>{}, column, out_tag, 1);
   };
   auto with_out = [&](auto column) {
@@ -948,6 +958,10 @@ void register_fp8_ops(pybind11::module_& m) {
   m.def("fp8_rows", &fp8_rows);
   m.def("fp8_both", &fp8_both);
   m.def("fp8_squares", &fp8_squares);
+  m.def("fp8_plan", [](int64_t M, int64_t N, int64_t K, bool column_scales, int sms) {
+    const ProductPlan plan = plan_product(M, N, K, column_scales, sms);
+    return std::make_tuple(plan.n, plan.splits);
+  });
   namespace py = pybind11;
   m.def("fp8_matmul", &fp8_matmul, py::arg("a"), py::arg("sa"), py::arg("b"), py::arg("sb"), py::arg("column_scales"), py::arg("out_bf16"), py::arg("addend"),
         py::arg("status"), py::arg("shape") = py::none());
