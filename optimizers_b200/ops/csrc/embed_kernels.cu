@@ -564,6 +564,14 @@ torch::Tensor embed_bwd(const torch::Tensor& ids, const torch::Tensor& dy, int64
   return out_bf16 && sliced ? out.to(torch::kBFloat16) : out;
 }
 
+// Kernels that embed_bwd launches for `tokens` tokens.
+int64_t embed_bwd_launches(int64_t tokens) {
+  if (tokens <= kFewTokens) return tokens > 0;
+  int64_t n = 0;
+  for (int64_t i0 = 0; i0 < tokens; i0 += kSortCapacity) n += tokens - i0 > kPiece ? 3 : 2;
+  return n;
+}
+
 void register_embed_ops(pybind11::module_& m) {
   m.def("embed_fwd", &embed_fwd);
   m.def("embed_bwd", &embed_bwd);

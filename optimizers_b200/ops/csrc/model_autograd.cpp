@@ -19,6 +19,7 @@ std::tuple<Tensor, Tensor, Tensor> add_norm_bwd(const Tensor& dy, const std::opt
                                                 bool want_dr);
 Tensor embed_fwd(const Tensor& ids, const Tensor& table, double scale, bool out_bf16);
 Tensor embed_bwd(const Tensor& ids, const Tensor& dy, int64_t V, double scale, bool out_bf16);
+int64_t embed_bwd_launches(int64_t tokens);
 std::tuple<Tensor, Tensor> fp8_rows(const Tensor& x);
 std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_both(const Tensor& x);
 std::tuple<Tensor, Tensor, Tensor> fp8_squares(const Tensor& w, bool transpose);
@@ -91,7 +92,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     ctx->saved_data["rows"] = table.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["bf16"] = is_bf16(table);
-    ++launches;
+    launches += i.numel() > 0;
     return embed_fwd(i, table.contiguous(), scale, out_bf16);
   }
 
@@ -99,7 +100,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const bool recorded = torch::GradMode::is_enabled();
     torch::NoGradGuard no_grad;
     const Tensor ids = ctx->get_saved_variables()[0];
-    launches += 3;
+    launches += embed_bwd_launches(ids.numel());
     Tensor dw = embed_bwd(ids, readable(grads[0]), ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["bf16"].toBool());
     return once(grads, {Tensor(), dw, Tensor(), Tensor()}, recorded, false);
   }

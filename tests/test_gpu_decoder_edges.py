@@ -135,3 +135,19 @@ def test_second_derivatives_are_never_lost_silently():
     for out, leaf in ((fp8.linear(x, w.detach()), x), (fused_ops.embedding(ids, table), table), (fused_ops.add_rms_norm(x, r, n)[1], x)):
         (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
         assert not g.requires_grad  # a constant
+
+
+@pytest.mark.parametrize("tokens, forward, backward", [(0, 0, 0), (1, 1, 1), (128, 1, 1), (129, 1, 3), (65536, 1, 3), (65537, 1, 5), (65600, 1, 6)])
+def test_launches_of_the_embedding_are_counted_as_they_are_made(tokens, forward, backward):
+    from torch.profiler import ProfilerActivity, profile
+
+    table, ids = torch.randn(50, 8, device="cuda", requires_grad=True), torch.arange(tokens, device="cuda") % 50
+    dy = torch.ones(tokens, 8, device="cuda")
+    y = fused_ops.embedding(ids, table)
+    for part, want in ((lambda: fused_ops.embedding(ids, table), forward), (lambda: y.backward(dy), backward)):
+        count = fused_ops.launches()
+        with profile(activities=[ProfilerActivity.CUDA]) as seen:
+            part()
+            torch.cuda.synchronize()
+        assert fused_ops.launches() - count == want
+        assert sum("embed_" in e.name for e in seen.events()) == want
