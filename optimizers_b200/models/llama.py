@@ -103,11 +103,9 @@ class _Layer(nn.Module):
     def _current(self, name: str) -> torch.Tensor | fp8.Weight:
         """The kept copy of a weight, or the weight itself if it has changed since."""
         weight, kept = getattr(self, name).weight, self._held.get(name)
-        if kept is None:
-            return weight
-        if kept.of(weight):
+        if kept is not None and kept.of(weight):
             return kept.value
-        del self._held[name]
+        self._held.pop(name, None)
         return weight
 
     def forward_fp8(self, branch: torch.Tensor | None, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):

@@ -151,3 +151,40 @@ def test_launches_of_the_embedding_are_counted_as_they_are_made(tokens, forward,
             torch.cuda.synchronize()
         assert fused_ops.launches() - count == want
         assert sum("embed_" in e.name for e in seen.events()) == want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float64])
+def test_clipping_refuses_gradients_with_gaps_that_share_memory(dtype):
+    from optimizers_b200 import clip_grad_norm_
+
+    whole = torch.ones(6, 8, device="cuda", dtype=dtype)
+    params = [torch.nn.Parameter(torch.zeros(6, 3, device="cuda", dtype=dtype)) for _ in range(2)]
+    params[0].grad, params[1].grad = whole[:, :3], whole[:, 2:5]
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_(params, 1.0)
+    assert bool((whole == 1).all())
+    params[1].grad = whole[:, 3:6]  # side by side
+    assert abs(float(clip_grad_norm_(params, 3.0)) - 6.0) < 1e-5
+    assert torch.allclose(whole[:, :6], torch.full_like(whole[:, :6], 0.5), rtol=2**-8) and bool((whole[:, 6:] == 1).all())
+
+
+def test_a_decoder_with_kept_weights_in_every_mode_and_in_a_graph():
+    """Weights kept in one mode serve the others; a captured evaluation is replayed with other tokens."""
+    from optimizers_b200.models import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    model = Llama(LlamaConfig(vocab_size=300, n_layer=2, n_head=2, d_model=128, d_ffn=256, fp8=True, fused_embedding=True)).cuda().eval()
+    ids = torch.randint(0, 300, (2, 17), device="cuda")
+    with torch.inference_mode(), torch.autocast("cuda", dtype=BF16):
+        want = model(ids)
+        model.hold_fp8_weights()
+        assert torch.equal(model(ids), want)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16):
+        assert torch.equal(model(ids), want) and all(len(layer._held) == 7 for layer in model.layers)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = model(ids)
+        ids.copy_(torch.randint(0, 300, (2, 17), device="cuda"))
+        graph.replay()
+        assert torch.equal(got, model(ids)) and not torch.equal(got, want)
+    fp8.check_status()
