@@ -263,7 +263,7 @@ def _sum_of(x: Tensor, residual: Tensor) -> Tensor:
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> Tensor:
     """``scale * weight[ids]`` in ``out_dtype`` (the table's by default), for integer ``ids`` of any shape and a table [V, C].
 
-    The gradient of the table is dense and summed in 32 bits, in the order of the tokens: the same inputs give the same bits.  On
+    The gradient of the table is dense and summed in 32 bits, in a fixed order: the same inputs give the same bits.  On
     the GPU, where a check would make the host wait, a token outside the table gives a row of NaN and takes no part in the
     gradient; PyTorch on the CPU raises ``IndexError``.
     """
