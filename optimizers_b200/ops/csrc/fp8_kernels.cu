@@ -234,8 +234,8 @@ fp8_tile_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
 //
 // What bounds it: the epilogue, about 950 clocks per group, of which 256 are multiply-adds (two warps per scheduler that run in step) and the
 // rest TMEM loads, barriers and their latencies; with a scale per row of B about 1550.  16384 x 2048 x 8192 by pairs: 160 us without
-// an epilogue, 184 without the multiply-adds, 242 as it is (2.27 PFLOP/s; 1.62 for the bf16 library product); 8192 x 16384 x 2048 with a
-// scale per row of B 397 us (1.38 PFLOP/s), 242 without the multiply-adds.  Sixteen epilogue warps with half the columns each spill
+// an epilogue, 184 without the multiply-adds, 238 as it is (2.31 PFLOP/s; 1.62 for the bf16 library product); 8192 x 16384 x 2048 with a
+// scale per row of B 389 us (1.41 PFLOP/s), 242 without the multiply-adds.  Sixteen epilogue warps with half the columns each spill
 // (429 us); reading TMEM as column pairs of eight rows took 305 us, single CTAs of 128 x 256 265 us.
 //
 // Products with few tiles are cut along K among the CTAs of a cluster, whose partial sums meet in distributed shared memory: each CTA adds
