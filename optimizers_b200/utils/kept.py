@@ -2,8 +2,8 @@
 
 A copy is good as long as its parameter is the same tensor in the same memory and counts no change since: PyTorch counts every operation that
 writes in place, ``load_state_dict`` and the optimizers' steps among them.  This package's kernels write parameters
-without that count, so the optimizers tell of it by ``written``.  What neither sees: writes through ``.data`` or a raw pointer, and the replay of a
-captured CUDA graph.
+without that count, so the optimizers tell of it by ``written``.  What neither sees: writes through ``.data``, a raw pointer or a collective, and the
+replay of a captured CUDA graph.
 """
 
 from __future__ import annotations
@@ -13,6 +13,7 @@ from collections.abc import Iterable
 from typing import Any
 
 from torch import Tensor
+from torch.nn import Parameter
 
 _alive: weakref.WeakSet[Kept] = weakref.WeakSet()
 
@@ -49,8 +50,8 @@ def any_alive() -> bool:
 
 
 def written(parameters: Iterable[Tensor]) -> None:
-    """A kernel has written these parameters."""
-    places = {p.data_ptr() for p in parameters}
+    """A kernel has written these parameters, or other parts of the memory that they lie in."""
+    storages = {p.untyped_storage().data_ptr() for p in parameters if type(p) in (Tensor, Parameter)}
     for kept in list(_alive):
-        if kept.place[0] in places:
+        if kept.memory.untyped_storage().data_ptr() in storages:
             kept.version = -1

@@ -193,3 +193,20 @@ def test_blocks_norm_and_embedding_sharded_on_their_own():
         s.bind(("127.0.0.1", 0))
         port = s.getsockname()[1]
     torch.multiprocessing.spawn(_sharded_worker, args=(port,), nprocs=2, join=True)
+
+
+def test_writes_to_the_memory_of_a_kept_weight_through_another_tensor():
+    """Parameters that are pieces of one buffer, which an optimizer's kernel writes as a whole."""
+    from optimizers_b200.utils import kept
+
+    model = _held_llama()
+    weight = model.layers[0].wq.weight
+    flat = torch.nn.Parameter(torch.cat([torch.zeros(7), weight.detach().flatten()]))
+    weight.data = flat.detach()[7:].view(32, 32)
+    with torch.no_grad():
+        model.hold_fp8_weights()
+        before = model(_IDX)
+        flat.data.neg_()
+        kept.written([flat, model.embed.weight])
+        assert not torch.equal(model(_IDX), before) and torch.equal(model(_IDX), _fresh(model))
+        assert sum(len(layer._held) for layer in model.layers) == 13
