@@ -24,6 +24,7 @@ def _variants(sizes):
     return {(column, *plan(*size, column, SMS)) for size in sizes for column in (False, True)}
 
 
+@pytest.mark.skipif(not build.available(), reason="the extension is not built")
 def test_the_sizes_reach_every_variant_that_any_size_reaches():
     rng = random.Random(0)
     anywhere = [tuple(int(math.exp(rng.uniform(0, math.log(20000)))) for _ in range(3)) for _ in range(20000)]
